@@ -38,6 +38,14 @@ enum {
     ORTMI_BF16 = 16,
 };
 
+/* Element types of a quantised key-value cache, ONNX codes: int8, packed int4 (two codes
+ * per byte, the even channel in the low nibble, each stored as code + 8), fp8 e4m3. */
+enum {
+    ORTMI_INT8 = 3,
+    ORTMI_F8E4M3 = 17,
+    ORTMI_INT4 = 22,
+};
+
 enum {
     ORTMI_OK = 0,
     ORTMI_E_INVALID = 1,     /* bad argument / unsupported form */
@@ -439,6 +447,71 @@ int ortmi_paged_attention(const void* query, const void* key, const void* value,
                           int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
                           int64_t v_head_size, float scale, int32_t dtype, void* workspace,
                           size_t workspace_bytes, void* stream);
+
+/*
+ * GroupQueryAttention over a quantised cache (inputs k_scale / v_scale, attributes
+ * k_quant_type / v_quant_type): past and present [batch, kv_num_heads, cap, head_size]
+ * hold codes of cache_type (ORTMI_INT8, ORTMI_F8E4M3: one byte each; ORTMI_INT4: rows of
+ * head_size / 2 bytes), a code standing for code * scale. k_scale / v_scale are device
+ * fp32: one number, or with *_per_channel != 0 [kv_num_heads, head_size].
+ *  - A new key row is (RMS-normalised,) rotated, divided by the scale and rounded to the
+ *    nearest code, ties to even, in 64 bits; a value row likewise without norm and
+ *    rotation. Codes past the range take its end, NaN is stored as 0.
+ *  - Every key and value, the new ones too, is read as the cache holds it.
+ * query / key / value, the shared and growing contracts, cos/sin, scale, q_norm_weight /
+ * k_norm_weight as ortmi_group_query_attention_ex; a growing cache needs present buffers
+ * of its own. seqlens_k (device int32 [batch], or NULL) gives each sequence's tokens less
+ * one, the new ones included, and is read by the kernels, clamped to
+ * [-1, total_sequence_length - 1]: n = seqlens_k[b] + 1 tokens, the new rows at positions
+ * max(n - seq_len, 0) on; rows at or past position n pad the batch: they give zero
+ * outputs and write nothing. Without it every sequence has total_sequence_length. The
+ * launches depend on total_sequence_length alone, so that with it set to an upper bound a
+ * call can be captured and replayed as seqlens_k grows.
+ * head_size a multiple of 16 up to 256; fp32, fp16 or bf16. The workspace holds
+ * ortmi_group_query_attention_quantized_workspace_size bytes, total_kv being
+ * valid_past + seq_len.
+ * No counterpart in the reference, whose claim declines these inputs.
+ */
+size_t ortmi_group_query_attention_quantized_workspace_size(int64_t batch, int64_t seq_len,
+                                                            int64_t num_heads,
+                                                            int64_t kv_num_heads,
+                                                            int64_t head_size, int64_t total_kv);
+int ortmi_group_query_attention_quantized(
+    const void* query, const void* key, const void* value, const void* past_key,
+    const void* past_value, int64_t past_cap, int32_t total_sequence_length,
+    const int32_t* seqlens_k, const void* cos_cache, const void* sin_cache, int64_t rotary_half,
+    int64_t max_pos, const void* q_norm_weight, const void* k_norm_weight, float qk_norm_epsilon,
+    const float* k_scale, const float* v_scale, int32_t k_per_channel, int32_t v_per_channel,
+    int32_t cache_type, void* output, void* present_key, void* present_value, int64_t batch,
+    int64_t seq_len, int64_t num_heads, int64_t kv_num_heads, int64_t head_size, float scale,
+    int32_t rotary_interleaved, int32_t dtype, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/*
+ * PagedAttention over quantised pages: key_cache / value_cache [num_blocks, block_size,
+ * kv_num_heads, head_size] hold codes as ortmi_group_query_attention_quantized has them,
+ * with the same scales, and new rows are quantised into the slots that block_table gives
+ * their positions. query, key, value, cum_seqlens, past_seqlens, block_table, max_context,
+ * cos/sin, head_sink [num_heads], q_norm_weight / k_norm_weight as ortmi_paged_attention;
+ * no slot_mapping, rotary_offset or LATENT layout. Every key and value, the new ones too,
+ * is read as the cache holds it; a position whose block the table does not hold
+ * (an id outside the cache) is neither written nor attended. Rows of output that belong to
+ * no sequence are left as they were. The workspace holds
+ * ortmi_paged_attention_quantized_workspace_size bytes.
+ */
+size_t ortmi_paged_attention_quantized_workspace_size(int64_t num_tokens, int64_t batch,
+                                                      int64_t num_heads, int64_t kv_num_heads,
+                                                      int64_t head_size, int64_t max_context);
+int ortmi_paged_attention_quantized(
+    const void* query, const void* key, const void* value, void* key_cache, void* value_cache,
+    int64_t num_blocks, int64_t block_size, const int32_t* cum_seqlens,
+    const int32_t* past_seqlens, const int32_t* block_table, int64_t batch, int64_t max_blocks,
+    int64_t num_tokens, int64_t max_context, const void* cos_cache, const void* sin_cache,
+    int64_t rotary_half, int64_t max_pos, int32_t rotary_interleaved, const void* head_sink,
+    const void* q_norm_weight, const void* k_norm_weight, float qk_norm_epsilon,
+    const float* k_scale, const float* v_scale, int32_t k_per_channel, int32_t v_per_channel,
+    int32_t cache_type, void* output, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
+    float scale, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * RotaryEmbedding (com.microsoft / ai.onnx), standalone.

@@ -22,6 +22,7 @@ KERNEL_LIB = os.path.join(LIB_DIR, "libortmi_kernels.so")
 EP_LIB = os.path.join(LIB_DIR, "libonnxruntime_mi355x_ep.so")
 
 ORTMI_F32, ORTMI_F16, ORTMI_BF16 = 1, 10, 16
+ORTMI_INT8, ORTMI_F8E4M3, ORTMI_INT4 = 3, 17, 22
 
 _kernels = None
 
@@ -100,6 +101,16 @@ SIGNATURES = {
         _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp,
         _i64, _i64, _i32, _i64, _vp, _vp, _vp, _vp, _f32, _vp, _i64, _i64, _i64, _i64, _f32,
         _i32, _vp, _sz, _vp]),
+    "ortmi_group_query_attention_quantized_workspace_size": (_sz, [_i64] * 6),
+    "ortmi_group_query_attention_quantized": (ctypes.c_int, [
+        _vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _f32, _vp, _vp,
+        _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _vp, _sz,
+        _vp]),
+    "ortmi_paged_attention_quantized_workspace_size": (_sz, [_i64] * 6),
+    "ortmi_paged_attention_quantized": (ctypes.c_int, [
+        _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp,
+        _i64, _i64, _i32, _vp, _vp, _vp, _f32, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _i64,
+        _f32, _i32, _vp, _sz, _vp]),
     "ortmi_rotary_embedding": (ctypes.c_int, [_vp, _vp, _i32, _vp, _vp, _i64, _vp, _i64, _i64,
                                               _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
     "ortmi_gather_block_quantized": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64,
@@ -135,9 +146,11 @@ from .ops import (  # noqa: E402,F401
     gather_block_quantized,
     group_query_attention,
     group_query_attention_decode_capturable,
+    group_query_attention_quantized,
     group_query_attention_sliding,
     matmul_nbits,
     paged_attention,
+    paged_attention_quantized,
     rotary_embedding,
     simplified_layer_norm,
     skip_simplified_layer_norm,

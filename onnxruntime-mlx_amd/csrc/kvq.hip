@@ -1,0 +1,386 @@
+// GroupQueryAttention and PagedAttention over quantised key-value caches: new rows into the
+// cache, attention for any head size, entry points.
+#include <algorithm>
+#include <cmath>
+
+#include "kvq.h"
+
+namespace ortmi {
+namespace kvq {
+
+// The last sequence that starts at or before token `tok`, and whether it has the token.
+__device__ __forceinline__ bool sequence_of_token(const Params& p, int tok, int& b, Seq& s) {
+    int lo = 0, hi = p.B;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.cum[mid] <= tok) lo = mid;
+        else hi = mid;
+    }
+    b = lo;
+    s = sequence<true>(p, lo);
+    return tok >= s.tok0 && tok < s.tok0 + s.rows;
+}
+
+// New keys and values into the cache: one wave per (token, kv head, key or value).
+template <bool PAGED>
+__global__ __launch_bounds__(256) void append_kernel(Params p) {
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int per = 2 * p.KV;
+    const int64_t tok = item / per;
+    if (tok >= p.T) return;
+    const int hv = (int)(item % per);
+    int b;
+    Seq s;
+    if constexpr (PAGED) {
+        if (!sequence_of_token(p, (int)tok, b, s)) return;
+    } else {
+        b = (int)(tok / p.S);
+        s = sequence<false>(p, b);
+    }
+    const int r = (int)tok - s.tok0;
+    if (r >= s.real) return;
+    append_row<PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV);
+}
+
+// Attention of one query row and head per workgroup, any head size that is a multiple of 16
+// up to 256: 16 teams of 16 lanes take every 16th key, a lane 1/16 of the channels; each
+// team keeps a running maximum and sum, joined at the end. The key scales are folded into
+// the query row and the value scales into the output, so the loop multiplies codes.
+constexpr int kTeams = 16, kMaxPerLane = 16;
+template <bool PAGED>
+__global__ __launch_bounds__(256) void row_kernel(Params p) {
+    __shared__ float sq[256];
+    __shared__ float so[kTeams][256];
+    __shared__ float sm[kTeams], sl[kTeams];
+    const int tok = blockIdx.x, head = blockIdx.y, hd = p.hd, tid = threadIdx.x;
+    const int h = head / (p.H / p.KV);
+    int b;
+    Seq s;
+    if constexpr (PAGED) {
+        if (!sequence_of_token(p, tok, b, s)) return;
+    } else {
+        b = tok / p.S;
+        s = sequence<false>(p, b);
+    }
+    const int r = tok - s.tok0;
+    const int64_t o0 = ((int64_t)tok * p.H + head) * hd;
+    if (r >= s.real) {  // a padded row
+        if (tid < hd) store_elem(p.out, o0 + tid, 0.f, p.dtype);
+        return;
+    }
+    const int64_t x0 = (int64_t)tok * p.q_tok + (int64_t)head * hd;
+    float rinv = 1.f;
+    if (p.qw) {
+        __shared__ float ssum[4];
+        float ss = 0.f;
+        if (tid < hd) {
+            const float x = load_elem(p.q, x0 + tid, p.dtype);
+            ss = x * x;
+        }
+        ss = wave_sum(ss);
+        if ((tid & 63) == 0) ssum[tid >> 6] = ss;
+        __syncthreads();
+        rinv = 1.f / sqrtf((ssum[0] + ssum[1] + ssum[2] + ssum[3]) / (float)hd + p.eps);
+    }
+    if (tid < hd) {
+        const int64_t prow = min((int64_t)(s.past + r), p.max_pos - 1) * p.half;
+        sq[tid] = query_elem(p, x0, prow, rinv, tid) * p.ks[p.k_chan ? h * hd + tid : 0] * p.scale;
+    }
+    __syncthreads();
+    const int team = tid >> 4, lane = tid & 15, per = hd / 16, c0 = lane * per;
+    float o[kMaxPerLane];
+    for (int i = 0; i < kMaxPerLane; ++i) o[i] = 0.f;
+    float m = -1e30f, l = 0.f;
+    const int rb = row_bytes(p.code, hd);
+    const int kend = s.keys_to(r, p.limit);
+    for (int j = team; j < kend; j += kTeams) {
+        const int64_t row = cache_row<PAGED>(p, b, h, j);
+        if (row < 0) continue;
+        const uint8_t* kr = p.kc + row * rb;
+        const uint8_t* vr = p.vc + row * rb;
+        float x = 0.f;
+        for (int i = 0; i < per; ++i) x += sq[c0 + i] * code_value(kr, c0 + i, p.code);
+        x = group_sum<16>(x);
+        const float mm = fmaxf(m, x), a = exp2f(m - mm), e = exp2f(x - mm);
+        l = l * a + e;
+        for (int i = 0; i < kMaxPerLane; ++i)
+            if (i < per) o[i] = o[i] * a + e * code_value(vr, c0 + i, p.code);
+        m = mm;
+    }
+    for (int i = 0; i < kMaxPerLane; ++i)
+        if (i < per) so[team][c0 + i] = o[i];
+    if (lane == 0) {
+        sm[team] = m;
+        sl[team] = l;
+    }
+    __syncthreads();
+    if (tid >= hd) return;
+    float mm = -1e30f;
+    if (p.sink) mm = load_elem(p.sink, head, p.dtype) * 1.44269504088896341f;
+    const float ms = mm;
+    for (int t = 0; t < kTeams; ++t) mm = fmaxf(mm, sm[t]);
+    float sum = p.sink ? exp2f(ms - mm) : 0.f, acc = 0.f;
+    for (int t = 0; t < kTeams; ++t) {
+        const float a = exp2f(sm[t] - mm);
+        sum += a * sl[t];
+        acc += a * so[t][tid];
+    }
+    const float v = sum != 0.f ? acc / sum * p.vs[p.v_chan ? h * hd + tid : 0] : 0.f;
+    store_elem(p.out, o0 + tid, v, p.dtype);
+}
+
+// Rows of the past into a present that is another buffer: `bytes` of each slab.
+__global__ __launch_bounds__(256) void copy_slabs_kernel(const uint8_t* __restrict__ src,
+                                                         uint8_t* __restrict__ dst,
+                                                         int64_t src_pitch, int64_t dst_pitch,
+                                                         int64_t bytes) {
+    const uint8_t* s = src + blockIdx.y * src_pitch;
+    uint8_t* d = dst + blockIdx.y * dst_pitch;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
+    if (i >= bytes) return;
+    if (i + 16 <= bytes &&
+        ((reinterpret_cast<uintptr_t>(s) | reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
+        *reinterpret_cast<uint4*>(d + i) = *reinterpret_cast<const uint4*>(s + i);
+    } else {
+        for (int64_t j = i; j < min(i + 16, bytes); ++j) d[j] = s[j];
+    }
+}
+
+static int copy_slabs(const void* src, void* dst, int64_t slabs, int64_t src_pitch,
+                      int64_t dst_pitch, int64_t bytes, hipStream_t st) {
+    if (slabs == 0 || bytes == 0) return ORTMI_OK;
+    const int64_t gx = (bytes + 4095) / 4096;
+    for (int64_t s0 = 0; s0 < slabs; s0 += 65535) {
+        const int64_t n = std::min<int64_t>(65535, slabs - s0);
+        hipLaunchKernelGGL(copy_slabs_kernel, dim3((unsigned)gx, (unsigned)n), dim3(256), 0, st,
+                           static_cast<const uint8_t*>(src) + s0 * src_pitch,
+                           static_cast<uint8_t*>(dst) + s0 * dst_pitch, src_pitch, dst_pitch,
+                           bytes);
+        if (int rc = check_launch("kv copy")) return rc;
+    }
+    return ORTMI_OK;
+}
+
+template <bool PAGED>
+static int attend(const Params& p, hipStream_t st) {
+    const int64_t items = (int64_t)p.T * 2 * p.KV;
+    hipLaunchKernelGGL((append_kernel<PAGED>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st,
+                       p);
+    if (int rc = check_launch("kv append")) return rc;
+    hipLaunchKernelGGL((row_kernel<PAGED>), dim3((unsigned)p.T, (unsigned)p.H), dim3(256), 0, st,
+                       p);
+    return check_launch("kv rows");
+}
+
+static bool code_of(int32_t cache_type, int& code) {
+    if (cache_type == ORTMI_INT8) code = kInt8;
+    else if (cache_type == ORTMI_INT4) code = kInt4;
+    else if (cache_type == ORTMI_F8E4M3) code = kFp8;
+    else return false;
+    return true;
+}
+
+}  // namespace kvq
+}  // namespace ortmi
+
+using namespace ortmi;
+
+// The checks that both operators share; `what` begins their messages.
+static int check_common(const std::string& what, int64_t num_heads, int64_t kv_num_heads,
+                        int64_t head_size, const void* cos_cache, const void* sin_cache,
+                        int64_t rotary_half, int64_t max_pos, const void* q_norm_weight,
+                        const void* k_norm_weight, const float* k_scale, const float* v_scale,
+                        int32_t cache_type, int32_t dtype) {
+    int code;
+    ORTMI_REQUIRE(num_heads > 0 && kv_num_heads > 0 && num_heads % kv_num_heads == 0 &&
+                      num_heads <= 65535,
+                  what + ": bad num_heads/kv_num_heads");
+    ORTMI_REQUIRE(head_size > 0 && head_size % 16 == 0 && head_size <= 256,
+                  what + ": head_size must be a multiple of 16 up to 256");
+    ORTMI_REQUIRE(dtype == ORTMI_F32 || dtype == ORTMI_F16 || dtype == ORTMI_BF16,
+                  what + ": dtype must be fp32, fp16 or bf16");
+    ORTMI_REQUIRE(kvq::code_of(cache_type, code), what + ": cache must be int8, int4 or fp8 e4m3");
+    ORTMI_REQUIRE(k_scale && v_scale, what + ": k_scale and v_scale must both be given");
+    ORTMI_REQUIRE((cos_cache != nullptr) == (sin_cache != nullptr),
+                  what + ": cos_cache and sin_cache must both be given");
+    ORTMI_REQUIRE(!cos_cache || (rotary_half > 0 && 2 * rotary_half <= head_size && max_pos > 0),
+                  what + ": rotary dims exceed head_size");
+    ORTMI_REQUIRE((q_norm_weight != nullptr) == (k_norm_weight != nullptr),
+                  what + ": q/k norm weights must both be given");
+    return ORTMI_OK;
+}
+
+extern "C" size_t ortmi_group_query_attention_quantized_workspace_size(
+    int64_t batch, int64_t seq_len, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
+    int64_t total_kv) {
+    (void)batch, (void)seq_len, (void)num_heads, (void)kv_num_heads, (void)head_size;
+    (void)total_kv;
+    return 0;
+}
+
+extern "C" int ortmi_group_query_attention_quantized(
+    const void* query, const void* key, const void* value, const void* past_key,
+    const void* past_value, int64_t past_cap, int32_t total_sequence_length,
+    const int32_t* seqlens_k, const void* cos_cache, const void* sin_cache, int64_t rotary_half,
+    int64_t max_pos, const void* q_norm_weight, const void* k_norm_weight, float qk_norm_epsilon,
+    const float* k_scale, const float* v_scale, int32_t k_per_channel, int32_t v_per_channel,
+    int32_t cache_type, void* output, void* present_key, void* present_value, int64_t batch,
+    int64_t seq_len, int64_t num_heads, int64_t kv_num_heads, int64_t head_size, float scale,
+    int32_t rotary_interleaved, int32_t dtype, void* workspace, size_t workspace_bytes,
+    void* stream) {
+    const std::string what = "GroupQueryAttention (quantized)";
+    if (int rc = check_common(what, num_heads, kv_num_heads, head_size, cos_cache, sin_cache,
+                              rotary_half, max_pos, q_norm_weight, k_norm_weight, k_scale, v_scale,
+                              cache_type, dtype))
+        return rc;
+    ORTMI_REQUIRE(batch >= 0 && seq_len >= 0 && past_cap >= 0, what + ": negative size");
+    ORTMI_REQUIRE(batch * seq_len < (1LL << 31) && past_cap + seq_len < (1LL << 31) &&
+                      batch * kv_num_heads < (1LL << 31),
+                  what + ": too many rows");
+    if (batch == 0 || seq_len == 0) return ORTMI_OK;
+    ORTMI_REQUIRE((key == nullptr) == (value == nullptr),
+                  what + ": key and value must both be given (or both absent, packed QKV)");
+    ORTMI_REQUIRE(query && output && present_key && present_value, what + ": null tensor");
+    // The KV contract of GroupQueryAttention (rust/src/ops/attention.rs:636-651).
+    int64_t vpast = (int64_t)total_sequence_length - seq_len;
+    bool shared = false;
+    if (vpast < 0 || vpast > past_cap) vpast = past_cap;
+    else shared = past_cap > vpast;
+    const int64_t pcap = shared ? past_cap : past_cap + seq_len;
+    ORTMI_REQUIRE(!shared || vpast + seq_len <= past_cap,
+                  what + ": total_sequence_length exceeds the KV buffer capacity");
+    ORTMI_REQUIRE(vpast == 0 || (past_key && past_value), what + ": null past");
+    ORTMI_REQUIRE(shared || past_cap == 0 ||
+                      (present_key != past_key && present_value != past_value),
+                  what + ": a growing cache needs present buffers of its own");
+    ORTMI_REQUIRE(!cos_cache || vpast + seq_len <= max_pos,
+                  what + ": position exceeds the cos/sin cache");
+    const int64_t hd = head_size;
+    hipStream_t st = as_stream(stream);
+    kvq::Params p{};
+    kvq::code_of(cache_type, p.code);
+    const size_t esize = dtype == ORTMI_F32 ? 4 : 2;
+    p.q = query;
+    if (key) {
+        p.k = key;
+        p.v = value;
+        p.q_tok = num_heads * hd;
+        p.kv_tok = kv_num_heads * hd;
+    } else {
+        p.k = static_cast<const char*>(query) + (size_t)(num_heads * hd) * esize;
+        p.v = static_cast<const char*>(p.k) + (size_t)(kv_num_heads * hd) * esize;
+        p.q_tok = p.kv_tok = (num_heads + 2 * kv_num_heads) * hd;
+    }
+    p.kc = static_cast<uint8_t*>(present_key);
+    p.vc = static_cast<uint8_t*>(present_value);
+    p.cap = pcap;
+    p.lens = seqlens_k;
+    p.vpast = (int)vpast;
+    p.S = (int)seq_len;
+    p.B = (int)batch;
+    p.H = (int)num_heads;
+    p.KV = (int)kv_num_heads;
+    p.hd = (int)hd;
+    p.T = (int)(batch * seq_len);
+    p.limit = (int)(vpast + seq_len);
+    p.cos = cos_cache;
+    p.sin = sin_cache;
+    p.half = (int)rotary_half;
+    p.interleaved = rotary_interleaved;
+    p.max_pos = max_pos;
+    p.qw = q_norm_weight;
+    p.kw = k_norm_weight;
+    p.eps = qk_norm_epsilon;
+    p.ks = k_scale;
+    p.vs = v_scale;
+    p.k_chan = k_per_channel;
+    p.v_chan = v_per_channel;
+    p.scale = (scale != 0.f ? scale : 1.0f / sqrtf((float)hd)) * 1.44269504088896341f;
+    p.dtype = dtype;
+    p.out = output;
+    (void)workspace, (void)workspace_bytes;
+    const int64_t rb = kvq::row_bytes(p.code, (int)hd), slabs = batch * kv_num_heads;
+    const int64_t kept = shared ? past_cap : vpast;  // rows of a past that is another buffer
+    const void* past[2] = {past_key, past_value};
+    void* present[2] = {present_key, present_value};
+    for (int i = 0; i < 2; ++i)
+        if (past[i] && present[i] != past[i])
+            if (int rc = kvq::copy_slabs(past[i], present[i], slabs, past_cap * rb, pcap * rb,
+                                         kept * rb, st))
+                return rc;
+    return kvq::attend<false>(p, st);
+}
+
+extern "C" size_t ortmi_paged_attention_quantized_workspace_size(
+    int64_t num_tokens, int64_t batch, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
+    int64_t max_context) {
+    (void)num_tokens, (void)batch, (void)num_heads, (void)kv_num_heads, (void)head_size;
+    (void)max_context;
+    return 0;
+}
+
+extern "C" int ortmi_paged_attention_quantized(
+    const void* query, const void* key, const void* value, void* key_cache, void* value_cache,
+    int64_t num_blocks, int64_t block_size, const int32_t* cum_seqlens,
+    const int32_t* past_seqlens, const int32_t* block_table, int64_t batch, int64_t max_blocks,
+    int64_t num_tokens, int64_t max_context, const void* cos_cache, const void* sin_cache,
+    int64_t rotary_half, int64_t max_pos, int32_t rotary_interleaved, const void* head_sink,
+    const void* q_norm_weight, const void* k_norm_weight, float qk_norm_epsilon,
+    const float* k_scale, const float* v_scale, int32_t k_per_channel, int32_t v_per_channel,
+    int32_t cache_type, void* output, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
+    float scale, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    const std::string what = "PagedAttention (quantized)";
+    if (int rc = check_common(what, num_heads, kv_num_heads, head_size, cos_cache, sin_cache,
+                              rotary_half, max_pos, q_norm_weight, k_norm_weight, k_scale, v_scale,
+                              cache_type, dtype))
+        return rc;
+    ORTMI_REQUIRE(batch > 0 && block_size > 0 && num_blocks > 0 && max_blocks > 0,
+                  what + ": bad cache or batch shape");
+    ORTMI_REQUIRE(num_tokens >= 0 && num_tokens < (1LL << 31), what + ": bad token count");
+    ORTMI_REQUIRE(batch < (1LL << 31) && block_size < (1LL << 31) && max_blocks < (1LL << 31),
+                  what + ": bad cache or batch shape");
+    ORTMI_REQUIRE(max_context > 0, what + ": max_context must be positive");
+    if (num_tokens == 0) return ORTMI_OK;
+    ORTMI_REQUIRE(query && key && value && key_cache && value_cache && cum_seqlens &&
+                      past_seqlens && block_table && output,
+                  what + ": null tensor");
+    kvq::Params p{};
+    kvq::code_of(cache_type, p.code);
+    p.q = query;
+    p.k = key;
+    p.v = value;
+    p.q_tok = num_heads * head_size;
+    p.kv_tok = kv_num_heads * head_size;
+    p.kc = static_cast<uint8_t*>(key_cache);
+    p.vc = static_cast<uint8_t*>(value_cache);
+    p.bt = block_table;
+    p.nblk = num_blocks;
+    p.blk = (int)block_size;
+    p.maxb = (int)max_blocks;
+    p.cum = cum_seqlens;
+    p.past = past_seqlens;
+    p.B = (int)batch;
+    p.H = (int)num_heads;
+    p.KV = (int)kv_num_heads;
+    p.hd = (int)head_size;
+    p.T = (int)num_tokens;
+    p.limit = (int)std::min<int64_t>({max_context, max_blocks * block_size, INT32_MAX});
+    p.cos = cos_cache;
+    p.sin = sin_cache;
+    p.half = (int)rotary_half;
+    p.interleaved = rotary_interleaved;
+    p.max_pos = max_pos;
+    p.qw = q_norm_weight;
+    p.kw = k_norm_weight;
+    p.eps = qk_norm_epsilon;
+    p.ks = k_scale;
+    p.vs = v_scale;
+    p.k_chan = k_per_channel;
+    p.v_chan = v_per_channel;
+    p.scale = (scale != 0.f ? scale : 1.0f / sqrtf((float)head_size)) * 1.44269504088896341f;
+    p.sink = head_sink;
+    p.dtype = dtype;
+    p.out = output;
+    (void)workspace, (void)workspace_bytes;
+    return kvq::attend<true>(p, as_stream(stream));
+}

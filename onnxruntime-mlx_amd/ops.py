@@ -11,7 +11,8 @@ import ctypes
 
 import torch
 
-from . import ORTMI_BF16, ORTMI_F16, ORTMI_F32, check, load_kernels
+from . import (ORTMI_BF16, ORTMI_F8E4M3, ORTMI_F16, ORTMI_F32, ORTMI_INT4, ORTMI_INT8, check,
+               load_kernels)
 
 _DT = {torch.float32: ORTMI_F32, torch.float16: ORTMI_F16, torch.bfloat16: ORTMI_BF16}
 
@@ -304,6 +305,222 @@ def paged_attention(query, key, value, key_cache, value_cache, cumulative_sequen
         _p(head_sink), _p(q_norm_weight), _p(k_norm_weight), float(qk_norm_epsilon), _p(out),
         num_heads, kv_num_heads, hd, vhd, float(scale), _dt(query), _p(ws), ws.numel(),
         _stream(stream)))
+    return out
+
+
+# ------------------------------------------------- quantised key-value caches
+# torch dtype of a cache -> (element code, channels per stored element).
+_CACHE = {torch.int8: (ORTMI_INT8, 1), torch.uint8: (ORTMI_INT4, 2),
+          torch.float8_e4m3fn: (ORTMI_F8E4M3, 1)}
+
+
+def _operand(what, name, t, dtype, device):
+    """Device address of an operand of the given dtype (None: absent)."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{what}: {name} must be on {device}, as the query is")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous")
+    return t.data_ptr()
+
+
+def _kv_scales(what, k_scale, v_scale, k_quant_type, v_quant_type, KV, hd, device):
+    """(k address, v address, k per channel, v per channel)."""
+    out = []
+    for name, s, kind in (("k", k_scale, k_quant_type), ("v", v_scale, v_quant_type)):
+        if kind not in ("PER_TENSOR", "PER_CHANNEL"):
+            raise ValueError(f"{what}: {name}_quant_type must be PER_TENSOR or PER_CHANNEL")
+        if s is None or s.numel() != (KV * hd if kind == "PER_CHANNEL" else 1):
+            raise ValueError(f"{what}: {name}_scale must hold one number, or with PER_CHANNEL "
+                             "kv_num_heads * head_size")
+        out.append((_operand(what, name + "_scale", s, torch.float32, device),
+                    int(kind == "PER_CHANNEL")))
+    return out[0][0], out[1][0], out[0][1], out[1][1]
+
+
+def _rotary_operands(what, do_rotary, cos_cache, sin_cache, hd, dtype, device):
+    """(cos address, sin address, half, rows)."""
+    if not do_rotary:
+        return None, None, 0, 0
+    if cos_cache is None or sin_cache is None or cos_cache.dim() != 2 or \
+            cos_cache.shape != sin_cache.shape or 2 * cos_cache.shape[1] > hd:
+        raise ValueError(f"{what}: do_rotary needs cos/sin caches [positions, at most "
+                         "head_size / 2]")
+    return (_operand(what, "cos_cache", cos_cache, dtype, device),
+            _operand(what, "sin_cache", sin_cache, dtype, device), cos_cache.shape[1],
+            cos_cache.shape[0])
+
+
+def _norm_operands(what, q_norm_weight, k_norm_weight, hd, dtype, device):
+    for w in (q_norm_weight, k_norm_weight):
+        if w is not None and w.numel() != hd:
+            raise ValueError(f"{what}: q/k norm weights must have head_size elements")
+    return (_operand(what, "q_norm_weight", q_norm_weight, dtype, device),
+            _operand(what, "k_norm_weight", k_norm_weight, dtype, device))
+
+
+def _own_device(what, query):
+    """The query's device, which has to be the current one (the stream's)."""
+    if not query.is_cuda:
+        raise ValueError("MI355X EP ops take device tensors")
+    if query.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: operands are on {query.device}, not on the current device")
+    return query.device
+
+
+def _own_workspace(what, workspace, nbytes, device):
+    """(address, bytes) of the caller's workspace, or of a new one (None: nothing needed)."""
+    if workspace is None:
+        workspace = _workspace(nbytes, device) if nbytes else None
+        return (workspace.data_ptr(), nbytes, workspace) if nbytes else (None, 0, None)
+    return _operand(what, "workspace", workspace, torch.uint8, device), workspace.numel(), workspace
+
+
+def group_query_attention_quantized(query, key, value, past_key, past_value, k_scale, v_scale,
+                                    seqlens_k, total_sequence_length, cos_cache=None,
+                                    sin_cache=None, *, num_heads, kv_num_heads,
+                                    k_quant_type="PER_TENSOR", v_quant_type="PER_TENSOR",
+                                    scale=0.0, do_rotary=0, rotary_interleaved=0,
+                                    present_key=None, present_value=None, q_norm_weight=None,
+                                    k_norm_weight=None, qk_norm_epsilon=1e-6, workspace=None,
+                                    stream=None):
+    """com.microsoft GroupQueryAttention with a quantised cache (inputs 12/13 k_scale and
+    v_scale, attributes k_quant_type / v_quant_type / kv_cache_bit_width).
+
+    past_key / past_value [B, KV, cap, hd] hold codes: torch.int8, torch.float8_e4m3fn, or
+    torch.uint8 with two 4-bit codes per byte ([B, KV, cap, hd / 2], the even channel in
+    the low nibble, stored as code + 8). k_scale / v_scale (float32) hold one number
+    ("PER_TENSOR") or one per (kv head, channel) ("PER_CHANNEL"). New rows are (normalised
+    and) rotated, divided by the scale and rounded to the nearest code; attention reads
+    every row, the new ones too, as the cache holds it. The shared and growing contracts
+    are those of group_query_attention; pass present_key=past_key /
+    present_value=past_value to append in place.
+
+    seqlens_k (int32 [B] on the device, or None) gives each sequence's tokens less one, at
+    most total_sequence_length - 1; rows past a sequence's end are padding (zero output,
+    nothing written). The launches depend on total_sequence_length alone: with it at an
+    upper bound, and a `workspace` (uint8) of the caller's, a call can be captured and
+    replayed as seqlens_k grows. Returns (output, present_key, present_value).
+    """
+    what = "GroupQueryAttention (quantized)"
+    device, dtype = _own_device(what, query), query.dtype
+    if query.dim() != 3 or (key is None) != (value is None):
+        raise ValueError(f"{what}: query must be [B, S, hidden], key and value both given or "
+                         "both absent (packed)")
+    B, S, hidden = query.shape
+    heads = num_heads + 2 * kv_num_heads if key is None else num_heads
+    hd = hidden // heads
+    if hd * heads != hidden:
+        raise ValueError(f"{what}: hidden size {hidden} is not a multiple of {heads} heads")
+    if past_key is None or past_key.dtype not in _CACHE:
+        raise TypeError(f"{what}: the cache must be int8, uint8 (packed int4) or float8_e4m3fn")
+    cdt = past_key.dtype
+    code, per = _CACHE[cdt]
+    if past_key.dim() != 4 or past_key.shape != past_value.shape or \
+            past_key.shape != (B, kv_num_heads, past_key.shape[2], hd // per):
+        raise ValueError(f"{what}: past key/value must be [batch, kv_num_heads, capacity, "
+                         "head_size (int4: / 2)]")
+    for name, t in (("key", key), ("value", value)):
+        if t is not None and t.shape != (B, S, kv_num_heads * hd):
+            raise ValueError(f"{what}: {name} must be [batch, seq_len, kv_num_heads * head_size]")
+    total, cap = int(total_sequence_length), past_key.shape[2]
+    shared, vp, pcap = gqa_contract(total, S, cap)
+    if shared and vp + S > cap:
+        raise ValueError(f"{what}: total_sequence_length exceeds the KV buffer capacity")
+    shape = (B, kv_num_heads, pcap, hd // per)
+    if present_key is None:
+        present_key = torch.empty(shape, dtype=cdt, device=device)
+    if present_value is None:
+        present_value = torch.empty(shape, dtype=cdt, device=device)
+    if present_key.shape != shape or present_value.shape != shape:
+        raise ValueError(f"{what}: present key/value have the wrong shape for the contract")
+    if seqlens_k is not None and seqlens_k.numel() != B:
+        raise ValueError(f"{what}: seqlens_k must have one value per sequence")
+    ks, vs, kc, vc = _kv_scales(what, k_scale, v_scale, k_quant_type, v_quant_type, kv_num_heads,
+                                hd, device)
+    rotary = _rotary_operands(what, do_rotary, cos_cache, sin_cache, hd, dtype, device)
+    norms = _norm_operands(what, q_norm_weight, k_norm_weight, hd, dtype, device)
+    out = torch.empty((B, S, num_heads * hd), dtype=dtype, device=device)
+    lib = load_kernels()
+    need = lib.ortmi_group_query_attention_quantized_workspace_size(
+        B, S, num_heads, kv_num_heads, hd, vp + S)
+    ws, ws_bytes, _keep = _own_workspace(what, workspace, need, device)
+    check(lib.ortmi_group_query_attention_quantized(
+        _operand(what, "query", query, dtype, device), _operand(what, "key", key, dtype, device),
+        _operand(what, "value", value, dtype, device),
+        _operand(what, "past_key", past_key, cdt, device),
+        _operand(what, "past_value", past_value, cdt, device), cap, total,
+        _operand(what, "seqlens_k", seqlens_k, torch.int32, device), *rotary, *norms,
+        qk_norm_epsilon, ks, vs, kc, vc, code, out.data_ptr(),
+        _operand(what, "present_key", present_key, cdt, device),
+        _operand(what, "present_value", present_value, cdt, device), B, S, num_heads,
+        kv_num_heads, hd, scale, rotary_interleaved, _dt(query), ws, ws_bytes, _stream(stream)))
+    return out, present_key, present_value
+
+
+def paged_attention_quantized(query, key, value, key_cache, value_cache, k_scale, v_scale,
+                              cumulative_sequence_length, past_seqlens, block_table,
+                              cos_cache=None, sin_cache=None, head_sink=None, q_norm_weight=None,
+                              k_norm_weight=None, *, num_heads, kv_num_heads,
+                              k_quant_type="PER_TENSOR", v_quant_type="PER_TENSOR", scale=0.0,
+                              do_rotary=0, rotary_interleaved=0, qk_norm_epsilon=1e-6,
+                              max_context=None, workspace=None, stream=None):
+    """PagedAttention over quantised pages (updated in place): paged_attention with
+    key_cache / value_cache [blocks, block, KV, hd] of codes and their scales as
+    group_query_attention_quantized has them.
+
+    All control tensors stay on the device. A position whose block the table does not hold
+    is neither written nor attended; rows of the output that belong to no sequence are not
+    written. Returns the output [T, H * hd].
+    """
+    what = "PagedAttention (quantized)"
+    device, dtype = _own_device(what, query), query.dtype
+    if key_cache.dtype not in _CACHE:
+        raise TypeError(f"{what}: the cache must be int8, uint8 (packed int4) or float8_e4m3fn")
+    cdt = key_cache.dtype
+    code, per = _CACHE[cdt]
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape or \
+            key_cache.shape[2] != kv_num_heads:
+        raise ValueError(f"{what}: caches must be [blocks, block, kv_num_heads, head_size "
+                         "(int4: / 2)]")
+    nblk, blk, KV, hd = key_cache.shape[0], key_cache.shape[1], kv_num_heads, \
+        key_cache.shape[3] * per
+    T = query.shape[0]
+    if query.shape != (T, num_heads * hd) or key.shape != (T, KV * hd) or \
+            value.shape != (T, KV * hd):
+        raise ValueError(f"{what}: query/key/value must be [tokens, heads * head_size]")
+    batch = cumulative_sequence_length.numel() - 1
+    if block_table.dim() != 2 or block_table.shape[0] != batch or past_seqlens.numel() != batch:
+        raise ValueError(f"{what}: past_seqlens [batch], block_table [batch, blocks] and "
+                         "cumulative_sequence_length [batch + 1] must agree")
+    if head_sink is not None and head_sink.numel() != num_heads:
+        raise ValueError(f"{what}: head_sink must have num_heads elements")
+    maxb = block_table.shape[1]
+    if max_context is None:
+        max_context = maxb * blk
+    ks, vs, kc, vc = _kv_scales(what, k_scale, v_scale, k_quant_type, v_quant_type, KV, hd, device)
+    rotary = _rotary_operands(what, do_rotary, cos_cache, sin_cache, hd, dtype, device)
+    norms = _norm_operands(what, q_norm_weight, k_norm_weight, hd, dtype, device)
+    out = torch.empty((T, num_heads * hd), dtype=dtype, device=device)
+    lib = load_kernels()
+    need = lib.ortmi_paged_attention_quantized_workspace_size(T, batch, num_heads, KV, hd,
+                                                              max_context)
+    ws, ws_bytes, _keep = _own_workspace(what, workspace, need, device)
+    i32 = torch.int32
+    check(lib.ortmi_paged_attention_quantized(
+        _operand(what, "query", query, dtype, device), _operand(what, "key", key, dtype, device),
+        _operand(what, "value", value, dtype, device),
+        _operand(what, "key_cache", key_cache, cdt, device),
+        _operand(what, "value_cache", value_cache, cdt, device), nblk, blk,
+        _operand(what, "cumulative_sequence_length", cumulative_sequence_length, i32, device),
+        _operand(what, "past_seqlens", past_seqlens, i32, device),
+        _operand(what, "block_table", block_table, i32, device), batch, maxb, T, max_context,
+        *rotary, rotary_interleaved, _operand(what, "head_sink", head_sink, dtype, device),
+        *norms, qk_norm_epsilon, ks, vs, kc, vc, code, out.data_ptr(), num_heads, KV, hd, scale,
+        _dt(query), ws, ws_bytes, _stream(stream)))
     return out
 
 
