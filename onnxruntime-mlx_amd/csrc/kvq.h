@@ -40,8 +40,17 @@ struct Params {
     const void* sink;           // [H], or null
     int dtype, code;
     void* out;                  // [T, H * hd]
-    float* part;                // [T * H][nsplit][hd + 2]: output, maximum, sum
-    int nsplit, chunk;          // splits of the keys, `chunk` (a multiple of 128) each
+    // Ranges of `chunk` keys (a multiple of 128): nsplit of them at most. Rows over more than
+    // one leave outputs part [T * H][nsplit][hd], maxima and sums ml [T * H][nsplit][2].
+    int nsplit, chunk;
+    float *part, *ml;
+    int ntile;                  // slabs: tiles of a sequence's columns
+    int fused;                  // slabs: the tiles write the new rows themselves
+    int blk_shift;              // pages: log2(blk), or -1
+    int2* tiles;                // pages: (sequence, first column) of tiles of 64 columns
+    int max_tiles;
+    int* tile_count;
+    int tile_chunk, tile_nsplit;  // pages: ranges of those tiles, at most nsplit of them
 };
 
 __device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {

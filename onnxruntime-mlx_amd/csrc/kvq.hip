@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "kvq.h"
+#include "kvq_tile.h"
 
 namespace ortmi {
 namespace kvq {
@@ -21,10 +21,40 @@ __device__ __forceinline__ bool sequence_of_token(const Params& p, int tok, int&
     return tok >= s.tok0 && tok < s.tok0 + s.rows;
 }
 
-// New keys and values into the cache: one wave per (token, kv head, key or value).
+// The tiles of the sequences with more than 16 columns, in order, by one wave. Ranges
+// of tokens are clamped to the call's (sequence()), and at most max_tiles are written.
+__device__ void list_tiles(const Params& p) {
+    const int lane = threadIdx.x & 63, G = p.H / p.KV, w = page_width(p.dtype);
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int b = b0 + lane;
+        const int cols = b < p.B ? sequence<true>(p, b).rows * G : 0;
+        const int n = cols > 16 ? (cols + w - 1) / w : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += v;
+        }
+        const int first = base + incl - n;
+        for (int i = 0; i < n && first + i < p.max_tiles; ++i) p.tiles[first + i] = make_int2(b, w * i);
+        base += __shfl(incl, 63, 64);
+    }
+    if (lane == 0) *p.tile_count = min(base, p.max_tiles);
+}
+
+// New keys and values into the cache: one wave per (token, kv head, key or value). Pages: the
+// first workgroup lists the tiles.
 template <bool PAGED>
 __global__ __launch_bounds__(256) void append_kernel(Params p) {
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if constexpr (PAGED) {
+        if (blockIdx.x == 0) {
+            if (threadIdx.x < 64 && p.tiles) list_tiles(p);
+            return;
+        }
+        item -= 4;
+    }
     const int per = 2 * p.KV;
     const int64_t tok = item / per;
     if (tok >= p.T) return;
@@ -40,6 +70,61 @@ __global__ __launch_bounds__(256) void append_kernel(Params p) {
     const int r = (int)tok - s.tok0;
     if (r >= s.real) return;
     append_row<PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV);
+}
+
+// Joins the ranges of the rows whose tile had more than one: a wave per (token, head).
+template <bool PAGED>
+__global__ __launch_bounds__(256) void merge_kernel(Params p) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= (int64_t)p.T * p.H) return;
+    const int lane = threadIdx.x & 63, tok = (int)(row / p.H), head = (int)(row % p.H);
+    const int G = p.H / p.KV, h = head / G;
+    int b;
+    Seq s;
+    if constexpr (PAGED) {
+        if (!sequence_of_token(p, tok, b, s)) return;
+    } else {
+        b = tok / p.S;
+        s = sequence<false>(p, b);
+    }
+    const int r = tok - s.tok0, cols = s.rows * G;
+    if (r >= s.real) return;
+    const int w = PAGED ? (cols <= 16 ? 16 : page_width(p.dtype)) : tile_width(cols, p.dtype);
+    const int c0 = (r * G + head - h * G) / w * w;
+    const int kend = s.keys_to((min(c0 + w, cols) - 1) / G, p.limit);
+    const int chunk = PAGED && cols > 16 ? p.tile_chunk : p.chunk;
+    const int n = (kend + chunk - 1) / chunk;
+    if (n <= 1) return;
+    const float* ml = p.ml + row * p.nsplit * 2;
+    float top = kNone;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, ml[2 * i]);
+    top = wave_max(top);
+    float a = 1.f, sum = 0.f;
+    for (int i = lane; i < n; i += 64) sum += ml[2 * i + 1] * __builtin_amdgcn_exp2f(ml[2 * i] - top);
+    sum = wave_sum(sum);
+    if (PAGED && p.sink) {
+        const float sk = load_elem(p.sink, head, p.dtype) * 1.44269504088896341f;
+        const float mm = fmaxf(top, sk);
+        a = __builtin_amdgcn_exp2f(top - mm);
+        sum = sum * a + __builtin_amdgcn_exp2f(sk - mm + kPBase);
+    }
+    const float inv = sum != 0.f ? a / sum : 0.f;
+    float acc[2] = {0.f, 0.f};
+    const float* o = p.part + row * p.nsplit * p.hd;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float e = __builtin_amdgcn_exp2f(ml[2 * i] - top);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (64 * j + lane < p.hd) acc[j] += e * o[(int64_t)i * p.hd + 64 * j + lane];
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int ch = 64 * j + lane;
+        if (ch >= p.hd) break;
+        const float y = inv != 0.f ? acc[j] * inv * p.vs[p.v_chan ? h * p.hd + ch : 0] : 0.f;
+        store_elem(p.out, row * p.hd + ch, y, p.dtype);
+    }
 }
 
 // Attention of one query row and head per workgroup, any head size that is a multiple of 16
@@ -161,15 +246,79 @@ static int copy_slabs(const void* src, void* dst, int64_t slabs, int64_t src_pit
     return ORTMI_OK;
 }
 
+// Ranges of keys for `wgs` workgroups each over n keys: enough to fill the GPU, each a
+// multiple of 128 keys (a block of 32 for each wave).
+static void plan_ranges(int64_t wgs, int64_t n, int64_t target, int& nsplit, int& chunk) {
+    const int64_t blocks = std::max<int64_t>(1, (n + 127) / 128);
+    const int64_t want = std::min<int64_t>(blocks, std::max<int64_t>(1, target / std::max<int64_t>(1, wgs)));
+    // At most 2^22 keys: a range's bytes stay below 2^31.
+    const int64_t per = std::min<int64_t>((blocks + want - 1) / want, 1 << 15);
+    chunk = (int)per * 128;
+    nsplit = (int)((blocks + per - 1) / per);
+}
+
+static bool tile_head(int64_t hd) { return hd == 64 || hd == 96 || hd == 128; }
+static size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+static void plan_slabs(int64_t B, int64_t S, int64_t H, int64_t KV, int64_t n, int dtype,
+                       int& ntile, int& nsplit, int& chunk) {
+    const int64_t cols = S * (H / KV);
+    const int w = tile_width((int)std::min<int64_t>(cols, 1 << 20), dtype);
+    ntile = (int)((cols + w - 1) / w);
+    plan_ranges(B * KV * ntile, n, w == 16 ? 768 : 256, nsplit, chunk);
+}
+
+static void plan_pages(int64_t B, int64_t KV, int64_t n, int& nsplit, int& chunk) {
+    plan_ranges(B * KV, n, 4096, nsplit, chunk);
+}
+
+static int max_page_tiles(int64_t T, int64_t B, int64_t G, int w) { return (int)((T * G + w - 1) / w + B); }
+
+static size_t ranges_bytes(int64_t rows, int nsplit, int64_t hd) {
+    return nsplit > 1 ? align_up((size_t)rows * nsplit * hd * 4) + align_up((size_t)rows * nsplit * 8) : 0;
+}
+
+// The ranges' part of the workspace; returns what lies behind it.
+static char* place_ranges(Params& p, char* ws) {
+    if (p.nsplit > 1) {
+        const size_t rows = (size_t)p.T * p.H;
+        p.part = reinterpret_cast<float*>(ws);
+        p.ml = reinterpret_cast<float*>(ws + align_up(rows * p.nsplit * p.hd * 4));
+        ws += ranges_bytes((int64_t)rows, p.nsplit, p.hd);
+    }
+    return ws;
+}
+
+// On the matrix cores where head size and alignment allow 16-byte loads and pages are whole
+// numbers of key tiles, otherwise a workgroup per row.
 template <bool PAGED>
-static int attend(const Params& p, hipStream_t st) {
-    const int64_t items = (int64_t)p.T * 2 * p.KV;
-    hipLaunchKernelGGL((append_kernel<PAGED>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st,
-                       p);
-    if (int rc = check_launch("kv append")) return rc;
-    hipLaunchKernelGGL((row_kernel<PAGED>), dim3((unsigned)p.T, (unsigned)p.H), dim3(256), 0, st,
-                       p);
-    return check_launch("kv rows");
+static int attend(Params& p, hipStream_t st) {
+    uintptr_t bits = 0;
+    for (const void* x : {(const void*)p.kc, (const void*)p.vc, p.q, (const void*)p.out, p.qw})
+        bits |= reinterpret_cast<uintptr_t>(x);
+    const bool tiles = tile_head(p.hd) && (bits & 15) == 0 &&
+                       (!PAGED || (p.blk % 16 == 0 && p.nblk <= INT32_MAX / p.blk));
+    if (!tiles) p.tiles = nullptr;
+    p.fused = !PAGED && tiles && p.ntile == 1;
+    if (!p.fused) {
+        const int64_t items = (int64_t)p.T * 2 * p.KV;
+        hipLaunchKernelGGL((append_kernel<PAGED>), dim3((unsigned)((items + 3) / 4 + (PAGED ? 1 : 0))),
+                           dim3(256), 0, st, p);
+        if (int rc = check_launch("kv append")) return rc;
+    }
+    if (!tiles) {
+        hipLaunchKernelGGL((row_kernel<PAGED>), dim3((unsigned)p.T, (unsigned)p.H), dim3(256), 0,
+                           st, p);
+        return check_launch("kv rows");
+    }
+    int rc;
+    if (p.code == kInt8) rc = tiles_int8(p, PAGED, st);
+    else if (p.code == kInt4) rc = tiles_int4(p, PAGED, st);
+    else rc = tiles_fp8(p, PAGED, st);
+    if (rc || p.nsplit == 1) return rc;
+    hipLaunchKernelGGL((merge_kernel<PAGED>), dim3((unsigned)(((int64_t)p.T * p.H + 3) / 4)),
+                       dim3(256), 0, st, p);
+    return check_launch("kv merge");
 }
 
 static bool code_of(int32_t cache_type, int& code) {
@@ -213,9 +362,17 @@ static int check_common(const std::string& what, int64_t num_heads, int64_t kv_n
 extern "C" size_t ortmi_group_query_attention_quantized_workspace_size(
     int64_t batch, int64_t seq_len, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
     int64_t total_kv) {
-    (void)batch, (void)seq_len, (void)num_heads, (void)kv_num_heads, (void)head_size;
-    (void)total_kv;
-    return 0;
+    if (batch <= 0 || seq_len <= 0 || kv_num_heads <= 0 || num_heads < kv_num_heads ||
+        !kvq::tile_head(head_size))
+        return 0;
+    size_t most = 0;  // over the types: fp32 has tiles of its own
+    for (int dtype : {ORTMI_F32, ORTMI_F16}) {
+        int ntile, nsplit, chunk;
+        kvq::plan_slabs(batch, seq_len, num_heads, kv_num_heads, total_kv, dtype, ntile, nsplit,
+                        chunk);
+        most = std::max(most, kvq::ranges_bytes(batch * seq_len * num_heads, nsplit, head_size));
+    }
+    return most;
 }
 
 extern "C" int ortmi_group_query_attention_quantized(
@@ -234,7 +391,7 @@ extern "C" int ortmi_group_query_attention_quantized(
                               cache_type, dtype))
         return rc;
     ORTMI_REQUIRE(batch >= 0 && seq_len >= 0 && past_cap >= 0, what + ": negative size");
-    ORTMI_REQUIRE(batch * seq_len < (1LL << 31) && past_cap + seq_len < (1LL << 31) &&
+    ORTMI_REQUIRE(batch * seq_len * num_heads < (1LL << 31) && past_cap + seq_len < (1LL << 31) &&
                       batch * kv_num_heads < (1LL << 31),
                   what + ": too many rows");
     if (batch == 0 || seq_len == 0) return ORTMI_OK;
@@ -298,7 +455,15 @@ extern "C" int ortmi_group_query_attention_quantized(
     p.scale = (scale != 0.f ? scale : 1.0f / sqrtf((float)hd)) * 1.44269504088896341f;
     p.dtype = dtype;
     p.out = output;
-    (void)workspace, (void)workspace_bytes;
+    kvq::plan_slabs(batch, seq_len, num_heads, kv_num_heads, vpast + seq_len, dtype, p.ntile,
+                    p.nsplit, p.chunk);
+    if (!kvq::tile_head(hd)) p.nsplit = 1;
+    const size_t need = kvq::ranges_bytes(batch * seq_len * num_heads, p.nsplit, hd);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(ORTMI_E_WORKSPACE, what + ": workspace too small");
+    ORTMI_REQUIRE(!need || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+                  what + ": workspace must be 16-byte aligned");
+    kvq::place_ranges(p, static_cast<char*>(workspace));
     const int64_t rb = kvq::row_bytes(p.code, (int)hd), slabs = batch * kv_num_heads;
     const int64_t kept = shared ? past_cap : vpast;  // rows of a past that is another buffer
     const void* past[2] = {past_key, past_value};
@@ -314,9 +479,13 @@ extern "C" int ortmi_group_query_attention_quantized(
 extern "C" size_t ortmi_paged_attention_quantized_workspace_size(
     int64_t num_tokens, int64_t batch, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
     int64_t max_context) {
-    (void)num_tokens, (void)batch, (void)num_heads, (void)kv_num_heads, (void)head_size;
-    (void)max_context;
-    return 0;
+    if (num_tokens <= 0 || batch <= 0 || kv_num_heads <= 0 || num_heads < kv_num_heads ||
+        !kvq::tile_head(head_size))
+        return 0;
+    int nsplit, chunk;
+    kvq::plan_pages(batch, kv_num_heads, max_context, nsplit, chunk);
+    return kvq::ranges_bytes(num_tokens * num_heads, nsplit, head_size) +
+           (size_t)(kvq::max_page_tiles(num_tokens, batch, num_heads / kv_num_heads, 32) + 1) * 8;
 }
 
 extern "C" int ortmi_paged_attention_quantized(
@@ -340,6 +509,7 @@ extern "C" int ortmi_paged_attention_quantized(
     ORTMI_REQUIRE(batch < (1LL << 31) && block_size < (1LL << 31) && max_blocks < (1LL << 31),
                   what + ": bad cache or batch shape");
     ORTMI_REQUIRE(max_context > 0, what + ": max_context must be positive");
+    ORTMI_REQUIRE(num_tokens * num_heads + 64 * batch < (1LL << 31), what + ": too many rows");
     if (num_tokens == 0) return ORTMI_OK;
     ORTMI_REQUIRE(query && key && value && key_cache && value_cache && cum_seqlens &&
                       past_seqlens && block_table && output,
@@ -381,6 +551,26 @@ extern "C" int ortmi_paged_attention_quantized(
     p.sink = head_sink;
     p.dtype = dtype;
     p.out = output;
-    (void)workspace, (void)workspace_bytes;
+    p.blk_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (block_size == 1LL << i) p.blk_shift = i;
+    p.nsplit = 1;
+    if (kvq::tile_head(head_size)) {
+        kvq::plan_pages(batch, kv_num_heads, max_context, p.nsplit, p.chunk);
+        p.max_tiles = kvq::max_page_tiles(num_tokens, batch, num_heads / kv_num_heads,
+                                          kvq::page_width(dtype));
+        const size_t need = kvq::ranges_bytes(num_tokens * num_heads, p.nsplit, head_size) +
+                            (size_t)(p.max_tiles + 1) * 8;
+        if (!workspace || workspace_bytes < need)
+            return fail(ORTMI_E_WORKSPACE, what + ": workspace too small");
+        ORTMI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+                      what + ": workspace must be 16-byte aligned");
+        char* ws = kvq::place_ranges(p, static_cast<char*>(workspace));
+        p.tile_count = reinterpret_cast<int*>(ws);
+        p.tiles = reinterpret_cast<int2*>(ws + 8);
+        // Tiles of 64 columns: ranges of four times the keys (their work fills the GPU sooner).
+        p.tile_chunk = (int)std::min<int64_t>(4LL * p.chunk, 1 << 23);
+        p.tile_nsplit = (p.nsplit + 3) / 4;
+    }
     return kvq::attend<true>(p, as_stream(stream));
 }
