@@ -601,6 +601,30 @@ int ortmi_argmax_rows(const void* x, int64_t* out, int64_t rows, int64_t cols, i
                       void* workspace, size_t workspace_bytes, void* stream);
 int ortmi_argmax_axis(const void* x, int64_t* out, int64_t outer, int64_t dim, int64_t inner,
                       int32_t select_last_index, int32_t dtype, void* stream);
+/*
+ * One token per row of logits [rows, cols], cols up to 262144: temperature, top-k, top-p
+ * and min-p, drawn with one given uniform number in [0, 1) per row. With
+ * w_i = exp((x_i - max) / temperature), in the order of falling logits (ties: the lower
+ * index first) the kept entries are the first top_k (<= 0: all), of those the shortest
+ * prefix that holds at least top_p of their weight (>= 1: all; at least one entry), of
+ * those the ones with w >= min_p (max w is 1; <= 0: all). ids (int64) receives the first
+ * index, in index order, at which the cumulative kept weight exceeds uniform times all of
+ * it; logprobs (fp32, may be NULL) the natural logarithm of its share. temperature <= 0,
+ * top_k = 1 or min_p > 1: the first of the largest logits, log-probability 0. NaN and
+ * -inf logits are never taken; a row of nothing else gives -1 and -inf. Weights are
+ * computed and summed in 64 bits, and the result does not depend on the order of the
+ * sums. temperature, top_k, top_p and min_p are device arrays [rows], or NULL: then the
+ * *_value of the same name serves every row. The greedy counterpart is
+ * ortmi_argmax_rows. The workspace holds ortmi_sample_rows_workspace_size bytes (NULL
+ * where that is 0).
+ */
+size_t ortmi_sample_rows_workspace_size(int64_t rows, int64_t cols);
+int ortmi_sample_rows(const void* logits, const float* uniform, const float* temperature,
+                      const int32_t* top_k, const float* top_p, const float* min_p,
+                      float temperature_value, int32_t top_k_value, float top_p_value,
+                      float min_p_value, int64_t* ids, float* logprobs, int64_t rows,
+                      int64_t cols, int32_t dtype, void* workspace, size_t workspace_bytes,
+                      void* stream);
 int ortmi_cast(const void* x, int32_t src_dtype, void* y, int32_t dst_dtype, int64_t n,
                void* stream);
 

@@ -124,6 +124,9 @@ SIGNATURES = {
     "ortmi_argmax_rows_workspace_size": (_sz, [_i64, _i64]),
     "ortmi_argmax_rows": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _sz, _vp]),
     "ortmi_argmax_axis": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "ortmi_sample_rows_workspace_size": (_sz, [_i64, _i64]),
+    "ortmi_sample_rows": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _f32,
+                                         _vp, _vp, _i64, _i64, _i32, _vp, _sz, _vp]),
     "ortmi_cast": (ctypes.c_int, [_vp, _i32, _vp, _i32, _i64, _vp]),
 }
 
@@ -152,6 +155,7 @@ from .ops import (  # noqa: E402,F401
     paged_attention,
     paged_attention_quantized,
     rotary_embedding,
+    sample_rows,
     simplified_layer_norm,
     skip_simplified_layer_norm,
 )

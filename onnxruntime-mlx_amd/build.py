@@ -25,7 +25,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 KERNEL_SOURCES = ["runtime.hip", "mnb.hip", "mnb_blk.hip", "mnb_gemm.hip", "attention.hip",
                   "attn_tile.hip", "norm.hip", "decode_step.hip", "gqa_ext.hip", "kvq.hip",
-                  "kvq_int8.hip", "kvq_int4.hip", "kvq_fp8.hip"]
+                  "kvq_int8.hip", "kvq_int4.hip", "kvq_fp8.hip", "sample.hip"]
 EP_SOURCES = ["ep/ep.cpp", "ep/graph.cpp", "ep/fuse.cpp", "ep/plan.cpp"]
 
 HIP_FLAGS = [

@@ -585,3 +585,54 @@ def skip_simplified_layer_norm(x, skip, gamma, bias=None, *, epsilon=1e-6, strea
                                         x.numel() // D, D, float(epsilon), _dt(x),
                                         _stream(stream)))
     return y, r
+
+
+# -------------------------------------------------------------------- Sampling
+def sample_rows(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                workspace=None, stream=None):
+    """One token per row of logits [..., V] (V up to 262144), drawn with one given uniform
+    number in [0, 1) per row: the sampling counterpart of the greedy argmax.
+
+    w = exp((x - max) / temperature); kept are, in the order of falling logits (ties: the
+    lower index first), the first top_k (<= 0: all), of those the shortest prefix that
+    holds top_p of their weight (>= 1: all), of those the entries with w >= min_p (max w
+    is 1). The token is the first index at which the cumulative kept weight, in index
+    order, exceeds uniform times all of it. temperature <= 0 takes the first of the largest
+    logits. NaN and -inf are never taken; a row of nothing else gives -1. Each setting is a
+    number or a device tensor of one per row (float32; top_k int32). Returns (ids int64,
+    logprobs float32), shaped as logits without the last axis; logprobs are under the
+    distribution that was drawn from.
+    """
+    what = "Sample"
+    device = _own_device(what, logits)
+    if logits.dim() < 1:
+        raise ValueError(f"{what}: logits must be [..., vocabulary]")
+    V = logits.shape[-1]
+    shape = logits.shape[:-1]
+    rows = shape.numel()
+    if uniform.numel() != rows:
+        raise ValueError(f"{what}: uniform must have one number per row")
+    arrays, numbers = [], []
+    for name, s, dtype, default in (("temperature", temperature, torch.float32, 1.0),
+                                    ("top_k", top_k, torch.int32, 0),
+                                    ("top_p", top_p, torch.float32, 1.0),
+                                    ("min_p", min_p, torch.float32, 0.0)):
+        if isinstance(s, torch.Tensor):
+            if s.numel() != rows:
+                raise ValueError(f"{what}: {name} must have one value per row")
+            arrays.append(_operand(what, name, s, dtype, device))
+            numbers.append(default)
+        else:
+            arrays.append(None)
+            numbers.append(s)
+    ids = torch.empty(shape, dtype=torch.int64, device=device)
+    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
+    lib = load_kernels()
+    ws, ws_bytes, _keep = _own_workspace(
+        what, workspace, lib.ortmi_sample_rows_workspace_size(rows, V), device)
+    check(lib.ortmi_sample_rows(
+        _operand(what, "logits", logits, logits.dtype, device),
+        _operand(what, "uniform", uniform, torch.float32, device), *arrays, *numbers,
+        ids.data_ptr(), logprobs.data_ptr(), rows, V, _dt(logits), ws, ws_bytes,
+        _stream(stream)))
+    return ids, logprobs

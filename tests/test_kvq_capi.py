@@ -71,3 +71,36 @@ def test_paged_refusals(lib, kw, word):
 
 def test_paged_empty_call(lib):
     assert paged(lib, T=0)[0] == 0
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dtype=3), "dtype"), (dict(rows=-1), "row count"), (dict(cols=0), "columns"),
+    (dict(cols=(1 << 18) + 1), "columns"), (dict(x=None), "null"), (dict(u=None), "null"),
+    (dict(ids=None), "null"),
+])
+def test_sample_refusals(lib, kw, word):
+    a = dict(x=P, u=P, ids=P, rows=2, cols=100, dtype=10)
+    a.update(kw)
+    rc = lib.ortmi_sample_rows(a["x"], a["u"], None, None, None, None, 1.0, 0, 1.0, 0.0, a["ids"],
+                               None, a["rows"], a["cols"], a["dtype"], None, 0, None)
+    assert rc == 1 and word in lib.ortmi_last_error().decode()
+
+
+def test_sample_empty_call(lib):
+    assert lib.ortmi_sample_rows(None, None, None, None, None, None, 1.0, 0, 1.0, 0.0, None, None,
+                                 0, 100, 10, None, 0, None) == 0
+
+
+def test_workspace_refusals(lib):
+    need = lib.ortmi_group_query_attention_quantized_workspace_size(1, 1, 4, 2, 64, 4096)
+    assert need > 0
+    kw = dict(cap=4096, total=4096, max_pos=4096)
+    for ws, n in ((P, need - 1), (None, need)):
+        rc, msg = gqa(lib, ws=ws, ws_bytes=n, **kw)
+        assert rc == 3 and "workspace" in msg
+    rc, msg = gqa(lib, ws=ctypes.c_void_p(4104), ws_bytes=need, **kw)
+    assert rc == 1 and "aligned" in msg
+    need = lib.ortmi_paged_attention_quantized_workspace_size(3, 2, 4, 2, 64, 64)
+    assert need > 0
+    rc, msg = paged(lib, ws_bytes=need - 1)
+    assert rc == 3 and "workspace" in msg
