@@ -616,7 +616,7 @@ int ortmi_argmax_axis(const void* x, int64_t* out, int64_t outer, int64_t dim, i
  * sums. temperature, top_k, top_p and min_p are device arrays [rows], or NULL: then the
  * *_value of the same name serves every row. The greedy counterpart is
  * ortmi_argmax_rows. The workspace holds ortmi_sample_rows_workspace_size bytes
- * (95 KB for each of up to 1024 rows).
+ * (117 KB for each of up to 1024 rows).
  */
 size_t ortmi_sample_rows_workspace_size(int64_t rows, int64_t cols);
 int ortmi_sample_rows(const void* logits, const float* uniform, const float* temperature,

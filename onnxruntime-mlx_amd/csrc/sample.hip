@@ -10,15 +10,19 @@
 //
 // Four launches, the first three with several workgroups a row where rows are few:
 //   top_kernel   the largest logit of each slice of a row;
-//   hist_kernel  top-k: a histogram of the largest of every eight logits, over keys relative
-//                to the row's largest: k of those are above a border, so at least k logits
-//                are, and few more. Top-p without top-k: histograms of all logits' weights
-//                and counts. Neither, nor min-p: the weight of every 512 logits;
-//   list_kernel  the entries above the border that the histogram gives go to a list (8192 at
-//                most; of a wider nucleus the entries of the border's bin);
-//   pick_kernel  one workgroup a row: the exact borders by radix selection over ordered
-//                32-bit keys (11 + 11 + 10 bits) on the list, then the token by the kept
-//                weight of every 512 indices and, in the 512 that pass u, of every one.
+//   hist_kernel  top-k: a histogram of the largest of every eight logits, over bins of 2^-7
+//                octave: k of those are above a border, so at least k logits are, and few
+//                more. Top-p without top-k: histograms of all logits' weights and counts (of
+//                16-bit logits counts alone: a bin's weight is that of its few values times
+//                their counts, so that no logit needs an exponential of its own). Neither, nor
+//                min-p: the weight of every 512 logits;
+//   list_kernel  top-k and min-p: the entries above the border go to a list, 8192 at most.
+//                Top-p without top-k: those of the border's bin alone, and what lies above it
+//                as weight by 512 indices;
+//   pick_kernel  one workgroup a row: the exact borders on the list (by comparing each of up
+//                to 256 entries with each, else by radix selection over ordered 32-bit keys),
+//                then the token by the kept weight of every 512 indices and, in the 512 that
+//                pass u, of every one.
 // A row whose border lies too low for the list has its selection over all of the row.
 #include <algorithm>
 #include <cmath>
@@ -29,11 +33,13 @@ namespace ortmi {
 namespace sample {
 
 constexpr int kThreads = 1024, kWaves = 16, kBins = 2048, kVec = 8;
+constexpr int kSmall = 256;  // entries that are compared each with each
 constexpr int kBlock = 512, kBlocks = 512;  // indices summed together; 262144 columns
 constexpr int kList = 8192, kSlices = 32;
-constexpr int kBinShift = 16;  // of keys: 128 bins an octave, 16 octaves below the largest
+constexpr int kHist = 4096;  // bins of a row's histogram
 constexpr double kUnit = 17592186044416.0;  // 2^44
 constexpr uint32_t kNoKey = 0;              // -inf and NaN: never taken
+constexpr uint32_t kOver = 0xFFFFFFFFu;
 
 struct Entry {
     uint32_t key, index;
@@ -42,17 +48,15 @@ struct Entry {
 // What the launches leave for each other, one for each row.
 struct Record {
     uint32_t slice_top[kSlices];  // keys
-    unsigned long long mass[kBins];
-    uint32_t count[kBins];
+    unsigned long long mass[kHist];
+    uint32_t count[kHist];
     unsigned long long rest;      // weight below the bins
     unsigned long long block[kBlocks];
     unsigned long long mass_above, all;
     uint32_t listed;              // kOver: the list does not have what the row needs
-    uint32_t bin_only;            // the list holds the border's bin, mass_above lies above it
+    uint32_t high;                // bin only: the largest key of the border's bin
     Entry list[kList];
 };
-constexpr uint32_t kOver = 0xFFFFFFFFu;
-
 struct Params {
     const void* x;
     const float* uniform;
@@ -108,6 +112,46 @@ struct Weight {
         return __builtin_bit_cast(uint64_t, v) & 0xFFFFFFFFFFFFFull;
     }
     __device__ __forceinline__ uint64_t units(float x) const { return units_of(of(x)); }
+};
+
+// Bins of a row's histogram, from the largest logit down, 128 an octave. A largest that is
+// positive: 2048 bins (16 octaves) of positive logits, one of all between, 2047 of negative
+// ones from 8 octaves below the largest's magnitude (at least 2^-9) on. One that is not: one
+// of magnitudes below 2^-16, or the largest's, 4095 of larger ones.
+struct Bins {
+    int top;      // the largest's magnitude, in units of 2^16 of its bits
+    bool positive;
+    __device__ __forceinline__ Bins(uint32_t top_key)
+        : top((int)((__float_as_uint(value_of(top_key)) & 0x7FFFFFFFu) >> 16)),
+          positive(top_key > 0x80000000u) {}
+    __device__ __forceinline__ int low() const {
+        return positive ? max(top - 1024, 0x3B00) : max(top, 0x3780);
+    }
+    // The bin of values that have no bin of their own.
+    __device__ __forceinline__ uint32_t between() const { return positive ? 2048u : 0u; }
+    // NaN, -inf and what lies below the bins: kOver.
+    __device__ __forceinline__ uint32_t of(float x) const {
+        const uint32_t u = __float_as_uint(x + 0.f);
+        const int h = (int)((u & 0x7FFFFFFFu) >> 16), l = low(), base = (int)between();
+        const int neg = h < l ? base : base + 1 + h - l;
+        const int d = u >= 0x80000000u ? neg : (positive ? min(top - h, 2048) : 0);
+        return ((x > -INFINITY) & (d < kHist)) ? (uint32_t)d : kOver;
+    }
+    // The keys of bin d.
+    __device__ __forceinline__ void keys(int d, uint32_t& first, uint32_t& last) const {
+        auto pos = [](int h) { return 0x80000000u | ((uint32_t)h << 16); };
+        const int base = (int)between();
+        if (d < base) {
+            first = pos(max(top - d, 0));
+            last = first + 0xFFFFu;
+        } else if (d == base) {
+            first = ~pos(low()) + 1;
+            last = positive ? pos(max(top - 2047, 0)) - 1 : 0x80000000u;
+        } else {
+            last = ~pos(low() + d - base - 1);
+            first = last - 0xFFFFu;
+        }
+    }
 };
 
 struct Shared {
@@ -435,7 +479,6 @@ __device__ __forceinline__ uint32_t row_top(const Params& p, const Record& rec) 
 template <typename T, typename F>
 __device__ __forceinline__ void each_block(const Params& p, const Row<T>& row, F f) {
     const int end = min(((int)blockIdx.x + 1) * p.per, p.blocks);
-#pragma unroll 2
     for (int b = (int)blockIdx.x * p.per + (int)(threadIdx.x >> 6); b < end; b += kWaves) {
         const int i0 = b * kBlock + (int)(threadIdx.x & 63) * kVec;
         uint32_t w[Row<T>::kWords];
@@ -449,7 +492,7 @@ __global__ __launch_bounds__(kThreads) void top_kernel(Params p) {
     __shared__ float wave_top[kWaves];
     const Row<T> row(p, blockIdx.y);
     Record& rec = p.records[blockIdx.y];
-    for (int i = blockIdx.x * kThreads + threadIdx.x; i < kBins; i += gridDim.x * kThreads) {
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < kHist; i += gridDim.x * kThreads) {
         rec.mass[i] = 0;
         rec.count[i] = 0;
         if (i < kBlocks) rec.block[i] = 0;
@@ -472,11 +515,15 @@ __global__ __launch_bounds__(kThreads) void top_kernel(Params p) {
     }
 }
 
+// Values that a bin of 2^16 of fp32's bits holds: bfloat16 1, fp16 8 (fp32: weights are summed).
+template <typename T>
+constexpr int kFine = std::is_same<T, half_t>::value ? 8 : 1;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void hist_kernel(Params p) {
-    __shared__ uint64_t mass[kBins];
-    __shared__ uint32_t count[kBins];
-    __shared__ uint64_t wave_rest[kWaves];
+    constexpr bool kSums = sizeof(T) == 4;
+    __shared__ uint64_t mass[kSums ? kHist : 1];
+    __shared__ uint32_t count[kHist * kFine<T>];
     const Settings o(p, blockIdx.y);
     Record& rec = p.records[blockIdx.y];
     const uint32_t top_key = row_top(p, rec);
@@ -484,6 +531,7 @@ __global__ __launch_bounds__(kThreads) void hist_kernel(Params p) {
     if (top_key == kNoKey || o.greedy() || !(by_count || by_mass || o.all())) return;
     const Row<T> row(p, blockIdx.y);
     const Weight w = o.weight(top_key);
+    const Bins bins(top_key);
     if (!by_count && !by_mass) {
         each_block(p, row, [&](int b, int, const uint32_t (&v)[Row<T>::kWords]) {
             uint64_t m = 0;
@@ -497,47 +545,82 @@ __global__ __launch_bounds__(kThreads) void hist_kernel(Params p) {
         });
         return;
     }
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        mass[i] = 0;
-        count[i] = 0;
-    }
+    const int fine = by_mass ? kFine<T> : 1;
+    for (int i = threadIdx.x; i < kHist * fine; i += kThreads) count[i] = 0;
+    if (kSums && by_mass)
+        for (int i = threadIdx.x; i < kHist; i += kThreads) mass[i] = 0;
     __syncthreads();
-    uint64_t rest = 0;
     if (by_count) {
         each_block(p, row, [&](int, int, const uint32_t (&v)[Row<T>::kWords]) {
             float x = -INFINITY;
 #pragma unroll
             for (int e = 0; e < kVec; ++e) x = fmaxf(x, Row<T>::value(v, e));
-            const uint32_t d = (top_key - key_of(x)) >> kBinShift;
-            if (d < kBins) atomicAdd(&count[d], 1u);
+            const uint32_t d = bins.of(x);
+            if (d != kOver) atomicAdd(&count[d], 1u);
         });
-    } else {
-        each_block(p, row, [&](int, int, const uint32_t (&v)[Row<T>::kWords]) {
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                const float x = Row<T>::value(v, e);
-                const uint32_t k = key_of(x), d = (top_key - k) >> kBinShift;
-                const uint64_t m = k == kNoKey ? 0 : w.units(x);
-                rest += d < kBins ? 0 : m;
-                if (d < kBins) {
-                    atomicAdd(&count[d], 1u);
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&mass[d]), (unsigned long long)m);
-                }
-            }
-        });
-        rest = wave_sum_u64(rest);
-        if ((threadIdx.x & 63) == 0) wave_rest[threadIdx.x >> 6] = rest;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kHist; i += kThreads)
+            if (count[i]) atomicAdd(&rec.count[i], count[i]);
+        return;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads)
-        if (count[i]) {
-            atomicAdd(&rec.count[i], count[i]);
-            if (by_mass) atomicAdd(&rec.mass[i], (unsigned long long)mass[i]);
+    uint64_t rest = 0;
+    each_block(p, row, [&](int, int, const uint32_t (&v)[Row<T>::kWords]) {
+        uint32_t out = 0;  // elements without a bin
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            const float x = Row<T>::value(v, e);
+            const uint32_t d = bins.of(x);
+            // 16-bit values without a bin of their own share one: their weights are summed.
+            const bool sums = kSums || d == bins.between();
+            if (d != kOver) {
+                if (kFine<T> == 1 || sums) atomicAdd(&count[d * kFine<T>], 1u);
+                else atomicAdd(&count[d * kFine<T> + ((__float_as_uint(x) >> 13) & 7u)], 1u);
+                if constexpr (kSums)
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&mass[d]), (unsigned long long)w.units(x));
+            }
+            out |= (!kSums && d != kOver && sums) || (d == kOver && x > -INFINITY) ? 1u << e : 0u;
         }
-    if (by_mass && threadIdx.x == 0) {
-        rest = 0;
-        for (int i = 0; i < kWaves; ++i) rest += wave_rest[i];
-        if (rest) atomicAdd(&rec.rest, (unsigned long long)rest);
+        while (__any(out != 0)) {  // few: one a lane and turn
+            if (out) {
+                const int e = __builtin_ctz(out);
+                out &= out - 1;
+                float x = 0.f;
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) x = j == e ? Row<T>::value(v, j) : x;
+                const uint32_t d = bins.of(x);
+                const uint64_t m = w.units(x);
+                if (d == kOver) rest += m;
+                else atomicAdd(&rec.mass[bins.between()], (unsigned long long)m);
+            }
+        }
+    });
+    rest = wave_sum_u64(rest);
+    if ((threadIdx.x & 63) == 0 && rest) atomicAdd(&rec.rest, (unsigned long long)rest);
+    __syncthreads();
+    for (int d = threadIdx.x; d < kHist; d += kThreads) {
+        uint32_t n = 0;
+        uint64_t m = 0;
+        if constexpr (kSums) {
+            n = count[d];
+            m = mass[d];
+        } else if (d == (int)bins.between()) {
+            n = count[d * kFine<T>];
+        } else {
+            // The bin's values, from bits whose upper half is the same.
+            uint32_t first, last;
+            bins.keys(d, first, last);
+            const uint32_t bits = __float_as_uint(value_of(first)) & 0xFFFF0000u;
+#pragma unroll
+            for (int j = 0; j < kFine<T>; ++j) {
+                const uint32_t c = count[d * kFine<T> + j];
+                if (c) m += c * w.units(__uint_as_float(bits | ((uint32_t)j << 13)));
+                n += c;
+            }
+        }
+        if (n) {
+            atomicAdd(&rec.count[d], n);
+            if (m) atomicAdd(&rec.mass[d], (unsigned long long)m);
+        }
     }
 }
 
@@ -549,15 +632,21 @@ __global__ __launch_bounds__(kThreads) void list_kernel(Params p) {
     const uint32_t top_key = row_top(p, rec);
     if (top_key == kNoKey || (o.all() && !o.greedy())) return;
     const int tid = threadIdx.x;
-    uint32_t low = top_key, high = 0xFFFFFFFFu, bin_only = 0;  // keys low .. high are listed
+    const bool by_mass = !o.greedy() && o.by_mass();
+    uint32_t low = top_key, high = kOver;  // keys low .. high are listed
     bool over = false;
     uint64_t all = 0, mass_above = 0;
-    if (!o.greedy() && (o.by_count() || o.by_mass())) {
-        const bool by_mass = o.by_mass();
-        const uint32_t c0 = rec.count[2 * tid], c1 = rec.count[2 * tid + 1];
-        const uint64_t m0 = by_mass ? rec.mass[2 * tid] : 0, m1 = by_mass ? rec.mass[2 * tid + 1] : 0;
-        uint32_t c = c0 + c1, call;
-        uint64_t m = m0 + m1, mall;
+    if (!o.greedy() && (o.by_count() || by_mass)) {
+        constexpr int kPer = kHist / kThreads;
+        uint32_t n[kPer], c = 0, call;
+        uint64_t v[kPer], m = 0, mall;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            n[i] = rec.count[kPer * tid + i];
+            v[i] = by_mass ? rec.mass[kPer * tid + i] : 0;
+            c += n[i];
+            m += v[i];
+        }
         if (tid == 0) sh.bin = kOver;
         block_scan(sh, c, m, call, mall);
         all = mall + rec.rest;
@@ -566,22 +655,22 @@ __global__ __launch_bounds__(kThreads) void list_kernel(Params p) {
         auto reached = [&](uint32_t cc, uint64_t mm) {
             return by_mass ? cc > 0 && (double)mm >= target : cc >= (uint32_t)o.top_k;
         };
-        if (!reached(c, m) && reached(c + c0 + c1, m + m0 + m1)) {
-            const bool second = !reached(c + c0, m + m0);
-            sh.bin = 2 * tid + (second ? 1 : 0);
-            sh.mass_above = second ? m + m0 : m;
-            sh.above = c + c0 + (second ? c1 : 0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (!reached(c, m) && reached(c + n[i], m + v[i])) {
+                sh.bin = kPer * tid + i;
+                sh.mass_above = m;
+            }
+            c += n[i];
+            m += v[i];
         }
         __syncthreads();
-        const uint32_t bin = sh.bin;
-        over = bin == kOver;
+        over = sh.bin == kOver;
         mass_above = sh.mass_above;
-        const uint64_t down = ((uint64_t)bin + 1) << kBinShift;
-        low = top_key >= down ? top_key - (uint32_t)down + 1 : kNoKey + 1;
-        if (by_mass && !over && sh.above > kList) {
-            bin_only = 1;
-            high = top_key - (bin << kBinShift);
-        }
+        uint32_t last = kOver;
+        if (!over) Bins(top_key).keys((int)sh.bin, low, last);
+        low = max(low, kNoKey + 1);
+        if (by_mass) high = last;
     } else if (!o.greedy()) {
         // Above the border of min-p, a little lowered: the weights decide.
         const double t = (double)value_of(top_key) +
@@ -593,28 +682,48 @@ __global__ __launch_bounds__(kThreads) void list_kernel(Params p) {
     if (blockIdx.x == 0 && tid == 0) {
         rec.all = all;
         rec.mass_above = mass_above;
-        rec.bin_only = bin_only;
+        rec.high = high;
         if (over) rec.listed = kOver;
     }
     if (over) return;
     const Row<T> row(p, blockIdx.y);
-    each_block(p, row, [&](int, int i0, const uint32_t (&v)[Row<T>::kWords]) {
-        uint32_t k[kVec], n = 0;
+    const Weight w = o.weight(top_key);
+    const double min_p = o.min_p > 0.f ? (double)o.min_p : 0.0;
+    each_block(p, row, [&](int b, int i0, const uint32_t (&v)[Row<T>::kWords]) {
+        uint32_t in = 0, above = 0;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-            k[e] = key_of(Row<T>::value(v, e));
-            n += k[e] >= low && k[e] <= high ? 1u : 0u;
+            const uint32_t k = key_of(Row<T>::value(v, e));
+            in |= ((k >= low) & (k <= high)) ? 1u << e : 0u;
+            above |= k > high ? 1u << e : 0u;
         }
-        if (__any(n > 0)) {
-            if (n > 0) {
-                uint32_t at = atomicAdd(&rec.listed, n);
+        if (__any(in != 0)) {
+            if (in) {
+                uint32_t at = atomicAdd(&rec.listed, (uint32_t)__popc(in));
 #pragma unroll
                 for (int e = 0; e < kVec; ++e)
-                    if (k[e] >= low && k[e] <= high) {
-                        if (at < kList) rec.list[at] = Entry{k[e], (uint32_t)(i0 + e)};
+                    if (in >> e & 1u) {
+                        if (at < kList)
+                            rec.list[at] = Entry{key_of(Row<T>::value(v, e)), (uint32_t)(i0 + e)};
                         ++at;
                     }
             }
+        }
+        if (by_mass) {  // kept for sure, but for min-p: their weight
+            uint64_t m = 0;
+            while (__any(above != 0)) {
+                if (above) {
+                    const int e = __builtin_ctz(above);
+                    above &= above - 1;
+                    float x = 0.f;
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) x = j == e ? Row<T>::value(v, j) : x;
+                    const double d = w.of(x);
+                    m += d >= min_p ? Weight::units_of(d) : 0;
+                }
+            }
+            m = wave_sum_u64(m);
+            if ((tid & 63) == 0) rec.block[b] = m;
         }
     });
 }
@@ -667,18 +776,82 @@ __device__ __forceinline__ Kept borders(const A& acc, const Settings& o, const W
     return Kept{key, last};
 }
 
-// The token over `acc`; the kept weight is returned, the index left in sh.index.
-template <typename A>
-__device__ __forceinline__ uint64_t draw(const A& acc, const Settings& o, const Weight& w,
-                                         Shared& sh, const Kept& kept) {
-    const bool floor = o.min_p > 0.f;
-    const double min_p = (double)o.min_p;
-    return locate(acc, sh, (double)o.u, 0.0, [&](uint32_t k, int i) -> uint64_t {
+// The weight that an entry adds: its own where it is kept.
+struct Part {
+    Weight w;
+    Kept kept;
+    double min_p;  // (the largest weighs 1: it passes)
+    __device__ __forceinline__ uint64_t operator()(uint32_t k, int i) const {
         const bool in = (k > kept.key) | ((k == kept.key) & (i <= kept.last));
         if (!in) return 0;
-        const double v = w.of(value_of(k));  // (min_p keeps the largest: its weight is 1)
-        return floor & !(v >= min_p) ? 0 : Weight::units_of(v);
-    });
+        const double v = w.of(value_of(k));
+        return v >= min_p ? Weight::units_of(v) : 0;
+    }
+};
+
+// Top-p without top-k: what lies above the border's bin is summed by 512 indices already, the
+// bin's entries are listed, and the row has the one block that is looked at in the end.
+template <typename T>
+struct Above {
+    const Row<T>& row;
+    const List& list;
+    const Record& rec;
+    template <typename F>
+    __device__ __forceinline__ void sum_blocks(uint64_t* block, F part) const {
+        if (threadIdx.x < kBlocks) block[threadIdx.x] = rec.block[threadIdx.x];
+        __syncthreads();
+        list.sum_blocks(block, part);
+    }
+    template <typename F>
+    __device__ __forceinline__ void fill_block(uint32_t b, uint64_t* inside, F part) const {
+        row.fill_block(b, inside, part);
+    }
+};
+
+__device__ __forceinline__ uint64_t add_xor(uint64_t v, int x) {
+    const uint32_t lo = __shfl_xor((uint32_t)v, x, 64), hi = __shfl_xor((uint32_t)(v >> 32), x, 64);
+    return v + (((uint64_t)hi << 32) | lo);
+}
+
+// Lists of at most 256 entries, four threads an entry: its rank and the weight before it by
+// comparison with every other. Leaves the kept entries' weights in sh.mass[entry] (0: not
+// kept) and returns their sum. The weight before the first is mass_above; `all` as in borders.
+__device__ __forceinline__ uint64_t keep_small(const List& list, const Settings& o, const Weight& w,
+                                               Shared& sh, uint64_t all, uint64_t mass_above) {
+    const int a = threadIdx.x >> 2, part = threadIdx.x & 3, n = list.n;
+    const bool have = a < n;
+    const Entry me = list.e[have ? a : 0];
+    const double weight = have ? w.of(value_of(me.key)) : 0.0;
+    const uint64_t units = Weight::units_of(weight);
+    __syncthreads();
+    if (part == 0) sh.mass[a] = units;
+    __syncthreads();
+    uint32_t rank = 0;
+    uint64_t before = 0;
+    for (int i = part; i < n; i += 4) {
+        const Entry b = list.e[i];
+        const bool first = (b.key > me.key) | ((b.key == me.key) & (b.index < me.index));
+        rank += first ? 1u : 0u;
+        before += first ? sh.mass[i] : 0;
+    }
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+        rank += __shfl_xor(rank, x, 64);
+        before = add_xor(before, x);
+    }
+    const bool own = have & (part == 0);  // one thread of an entry's four counts it
+    const uint32_t k = o.top_k > 0 ? (uint32_t)o.top_k : kOver;
+    if (!all) all = block_sum(sh, (own & (rank < k)) ? units : 0);
+    before += mass_above;
+    // Selects, no branches: the compiler has lost the zero of an `if (!keep) units = 0` here.
+    const bool in_p = !(o.top_p < 1.f) | ((double)before < (double)o.top_p * (double)all);
+    const bool in_m = !(o.min_p > 0.f) | (weight >= (double)o.min_p);
+    const bool keep = own & (rank < k) & (((rank == 0) & (mass_above == 0)) | (in_p & in_m));
+    const uint64_t kept = keep ? units : 0;
+    const uint64_t total = block_sum(sh, kept);  // its barriers end the reading of sh.mass
+    if (part == 0) sh.mass[a] = kept;
+    __syncthreads();
+    return total;
 }
 
 template <typename T>
@@ -698,41 +871,64 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(Params p) {
         }
         return;
     }
-    const bool greedy = o.greedy();
+    const bool greedy = o.greedy(), by_mass = !greedy && o.by_mass();
     const Weight w = o.weight(top_key);
     const bool listed = (greedy || !o.all()) && rec.listed <= kList;
-    List list{entries, listed ? (int)rec.listed : 0};
+    const List list{entries, listed ? (int)rec.listed : 0};
     for (int i = tid; i < list.n; i += kThreads) entries[i] = rec.list[i];
+    if (tid == 0) sh.index = -1;
+    __syncthreads();
+    const double min_p = o.min_p > 0.f ? (double)o.min_p : 0.0;
     uint64_t total = 0;
     if (greedy) {
         auto first = [&](uint32_t k, int) -> uint64_t { return k == top_key ? 1 : 0; };
         if (listed) locate(list, sh, -1.0, 0.0, first);
         else locate(row, sh, -1.0, 0.0, first);
     } else if (o.all()) {
-        // The blocks' weights are there.
-        __syncthreads();
-        if (tid < kBlocks) {
-            sh.block[tid] = rec.block[tid];
-            sh.inside[tid] = 0;
+        const List none{entries, 0};
+        total = locate(Above<T>{row, none, rec}, sh, (double)o.u, 0.0,
+                       Part{w, Kept{kNoKey + 1, row.cols}, 0.0});
+    } else if (listed && list.n <= kSmall) {
+        const uint64_t kept = keep_small(list, o, w, sh, rec.all, by_mass ? rec.mass_above : 0);
+        if (!by_mass) {
+            // Cumulative weights in index order, by comparison.
+            total = kept;
+            const int a = tid >> 2, part = tid & 3;
+            const uint64_t own = sh.mass[a];
+            const uint32_t index = entries[a < list.n ? a : 0].index;
+            uint64_t cum = 0;
+            for (int i = part; i < list.n; i += 4) cum += entries[i].index < index ? sh.mass[i] : 0;
+            cum = add_xor(add_xor(cum, 1), 2);
+            if (part == 0 && a < list.n && falls_on(cum, own, (double)o.u * (double)total, total))
+                sh.index = index;
+        } else {
+            // The last kept of the bin, in order: the border for the one block that is read.
+            __shared__ uint32_t low_key;
+            __shared__ int last;
+            if (tid == 0) {
+                low_key = kOver;
+                last = -1;
+            }
+            __syncthreads();
+            const bool mine = tid < list.n && sh.mass[tid] != 0;
+            const Entry e = entries[tid < list.n ? tid : 0];
+            if (mine) atomicMin(&low_key, e.key);
+            __syncthreads();
+            if (mine && e.key == low_key) atomicMax(&last, (int)e.index);
+            __syncthreads();
+            const Kept border{low_key == kOver ? rec.high : low_key, low_key == kOver ? -1 : last};
+            total = locate(Above<T>{row, list, rec}, sh, (double)o.u, 0.0, Part{w, border, min_p});
         }
-        __syncthreads();
-        double want = 0.0;
-        total = find_part(sh, sh.block, (double)o.u, 0, 0, true, want);
-        const uint32_t b = sh.hit;
-        const uint64_t before = sh.before;
-        row.fill_block(b, sh.inside, [&](uint32_t k, int) -> uint64_t {
-            return k == kNoKey ? 0 : w.units(value_of(k));
-        });
-        __syncthreads();
-        find_part(sh, sh.inside, 0.0, before, total, false, want);
-        if (tid == 0) sh.index = (int64_t)b * kBlock + sh.hit;
-    } else if (listed && !rec.bin_only) {
-        total = draw(list, o, w, sh, borders(list, o, w, sh, rec.all, 0, row.cols));
     } else if (listed) {
-        total = draw(row, o, w, sh, borders(list, o, w, sh, rec.all, rec.mass_above, row.cols));
+        const Kept border = borders(list, o, w, sh, rec.all, by_mass ? rec.mass_above : 0, row.cols);
+        const Part part{w, border, min_p};
+        if (by_mass) total = locate(Above<T>{row, list, rec}, sh, (double)o.u, 0.0, part);
+        else total = locate(list, sh, (double)o.u, 0.0, part);
     } else {
-        total = draw(row, o, w, sh, borders(row, o, w, sh, 0, 0, row.cols));
+        const Kept border = borders(row, o, w, sh, 0, 0, row.cols);
+        total = locate(row, sh, (double)o.u, 0.0, Part{w, border, min_p});
     }
+    __syncthreads();
     if (tid == 0) {
         const int64_t i = sh.index;
         p.ids[p.row0 + r] = i;
@@ -742,7 +938,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(Params p) {
     }
 }
 
-// Rows at a time: what bounds the workspace (95 KB a row).
+// Rows at a time: what bounds the workspace (117 KB a row).
 constexpr int64_t kRows = 1024;
 
 }  // namespace sample
