@@ -5,7 +5,7 @@
 // entries are the first k (top-k), of those the shortest prefix that holds p of their weight
 // (top-p), of those the entries with w >= min_p (min-p; max w is 1). The token is the first,
 // in index order, at which the kept weight exceeds u times all of it. Borders decide, so
-// weights are computed in 64 bits (2e-13 relative) and summed as integers in units of 2^-44:
+// weights are computed in 64 bits (2e-12 relative) and summed as integers in units of 2^-44:
 // a sum is then the same in whatever order its parts arrive.
 //
 // Four launches, the first three with several workgroups a row where rows are few:
@@ -82,30 +82,35 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// 2^z for z <= 0, within 2e-13 of it: the power series of exp to the tenth term on half a unit
-// around the next integer.
-__device__ __forceinline__ double exp2_64(double z) {
-    const double n = rint(z), t = (z - n) * 0.69314718055994530942;
-    double r = 1.0 / 3628800.0;
-    r = fma(r, t, 1.0 / 362880.0);
-    r = fma(r, t, 1.0 / 40320.0);
-    r = fma(r, t, 1.0 / 5040.0);
-    r = fma(r, t, 1.0 / 720.0);
-    r = fma(r, t, 1.0 / 120.0);
-    r = fma(r, t, 1.0 / 24.0);
-    r = fma(r, t, 1.0 / 6.0);
-    r = fma(r, t, 0.5);
-    r = fma(r, t, 1.0);
-    r = fma(r, t, 1.0);
-    return ldexp(r, (int)n);
+// Weights by 2^z = 2^n 2^(i/32) 2^r: the middle from a table in LDS, |r| <= 1/64 by the power
+// series of exp to the fourth term (1.2e-12 relative).
+constexpr int kTable = 32;
+
+// The table, before a barrier: exp's power series to the term of 2e-16 on [0, 1) by halves.
+__device__ __forceinline__ void fill_table(double* table) {
+    if (threadIdx.x < kTable) {
+        const double t = (double)threadIdx.x * (0.69314718055994530942 / (2 * kTable));
+        double r = 1.0;
+#pragma unroll
+        for (int i = 12; i >= 1; --i) r = fma(r, t * (1.0 / i), 1.0);
+        table[threadIdx.x] = r * r;  // exp(t)^2
+    }
 }
 
 struct Weight {
     double top, c;  // the row's maximum, log2(e) / T
-    // The largest weighs 1 (also an infinity, beside which all else weighs 0).
+    const double* table;
+    // The largest weighs 1 (an infinity as the largest finite: beside it all else weighs 0).
     __device__ __forceinline__ double of(float x) const {
-        const double z = ((double)x - top) * c;
-        return (double)x == top ? 1.0 : (z > -1000.0 ? exp2_64(z) : 0.0);
+        const double z = fmax(((double)fminf(x, 3.402823466e38f) - top) * c, -1000.0);
+        const double kd = fma(z, (double)kTable, 6755399441055744.0);  // 1.5 2^52: an integer's bits
+        const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, kd);
+        const double r = fma(kd - 6755399441055744.0, -1.0 / kTable, z);
+        double e = fma(r, 0.0096181291076284772, 0.055504108664821580);  // ln2^4 / 24, ln2^3 / 6
+        e = fma(r, e, 0.24022650695910071);
+        e = fma(r, e, 0.69314718055994531);
+        e = fma(r, e, 1.0);
+        return ldexp(e * table[k & (kTable - 1)], k >> 5);
     }
     __device__ static __forceinline__ uint64_t units_of(double w) {  // at most 2^44: exact in 2^52
         const double v = w * kUnit + 4503599627370496.0;
@@ -464,8 +469,9 @@ struct Settings {
     __device__ __forceinline__ bool by_count() const { return top_k > 0; }
     __device__ __forceinline__ bool by_mass() const { return top_k == 0 && top_p < 1.f; }
     __device__ __forceinline__ bool all() const { return top_k == 0 && !(top_p < 1.f) && !(min_p > 0.f); }
-    __device__ __forceinline__ Weight weight(uint32_t top_key) const {
-        return Weight{(double)value_of(top_key), 1.4426950408889634074 / (double)temperature};
+    __device__ __forceinline__ Weight weight(uint32_t top_key, const double* table) const {
+        return Weight{(double)fminf(value_of(top_key), 3.402823466e38f),
+                      1.4426950408889634074 / (double)temperature, table};
     }
 };
 
@@ -524,15 +530,18 @@ __global__ __launch_bounds__(kThreads) void hist_kernel(Params p) {
     constexpr bool kSums = sizeof(T) == 4;
     __shared__ uint64_t mass[kSums ? kHist : 1];
     __shared__ uint32_t count[kHist * kFine<T>];
+    __shared__ double table[kTable];
     const Settings o(p, blockIdx.y);
     Record& rec = p.records[blockIdx.y];
     const uint32_t top_key = row_top(p, rec);
     const bool by_count = o.by_count(), by_mass = o.by_mass();
     if (top_key == kNoKey || o.greedy() || !(by_count || by_mass || o.all())) return;
     const Row<T> row(p, blockIdx.y);
-    const Weight w = o.weight(top_key);
+    const Weight w = o.weight(top_key, table);
     const Bins bins(top_key);
+    fill_table(table);
     if (!by_count && !by_mass) {
+        __syncthreads();
         each_block(p, row, [&](int b, int, const uint32_t (&v)[Row<T>::kWords]) {
             uint64_t m = 0;
 #pragma unroll
@@ -627,10 +636,13 @@ __global__ __launch_bounds__(kThreads) void hist_kernel(Params p) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void list_kernel(Params p) {
     __shared__ Shared sh;
+    __shared__ double table[kTable];
     const Settings o(p, blockIdx.y);
     Record& rec = p.records[blockIdx.y];
     const uint32_t top_key = row_top(p, rec);
     if (top_key == kNoKey || (o.all() && !o.greedy())) return;
+    fill_table(table);
+    __syncthreads();
     const int tid = threadIdx.x;
     const bool by_mass = !o.greedy() && o.by_mass();
     uint32_t low = top_key, high = kOver;  // keys low .. high are listed
@@ -687,7 +699,7 @@ __global__ __launch_bounds__(kThreads) void list_kernel(Params p) {
     }
     if (over) return;
     const Row<T> row(p, blockIdx.y);
-    const Weight w = o.weight(top_key);
+    const Weight w = o.weight(top_key, table);
     const double min_p = o.min_p > 0.f ? (double)o.min_p : 0.0;
     each_block(p, row, [&](int b, int i0, const uint32_t (&v)[Row<T>::kWords]) {
         uint32_t in = 0, above = 0;
@@ -858,6 +870,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void pick_kernel(Params p) {
     __shared__ Shared sh;
     __shared__ Entry entries[kList];
+    __shared__ double table[kTable];
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const Settings o(p, r);
@@ -872,7 +885,8 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(Params p) {
         return;
     }
     const bool greedy = o.greedy(), by_mass = !greedy && o.by_mass();
-    const Weight w = o.weight(top_key);
+    const Weight w = o.weight(top_key, table);
+    fill_table(table);
     const bool listed = (greedy || !o.all()) && rec.listed <= kList;
     const List list{entries, listed ? (int)rec.listed : 0};
     for (int i = tid; i < list.n; i += kThreads) entries[i] = rec.list[i];
@@ -956,9 +970,10 @@ static int sample_rows(sample::Params p, int64_t rows, hipStream_t st) {
     p.blocks = (int)((p.cols + sample::kBlock - 1) / sample::kBlock);
     for (int64_t r0 = 0; r0 < rows; r0 += sample::kRows) {
         const int64_t n = std::min(sample::kRows, rows - r0);
-        // Slices of a row, whole rounds of a workgroup's 16 waves: one workgroup a CU in all.
+        // Slices of a row, whole rounds of a workgroup's 16 waves: two workgroups a CU, and four
+        // a row, so that rows whose settings ask for more work do not hold up the others.
         const int64_t rounds = (p.blocks + sample::kWaves - 1) / sample::kWaves;
-        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(device_cu_count() / n, rounds));
+        const int64_t want = std::min<int64_t>(std::max<int64_t>(4, 2 * device_cu_count() / n), rounds);
         const int64_t each = (rounds + want - 1) / want;
         p.per = (int)each * sample::kWaves;
         p.slices = (int)((rounds + each - 1) / each);

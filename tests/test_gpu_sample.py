@@ -1,5 +1,5 @@
 """Sampling on the GPU against numpy in 64 bits: tokens are equal, log-probabilities within
-the steps of fp32 that a value of theirs has (the weights are 2e-13 exact).
+the steps of fp32 that a value of theirs has (the weights are 2e-12 exact).
 
 A token can differ from the reference's where the uniform number, or a border of the kept
 entries, falls within the weights' error of a border between entries: about 1e-9 of the
@@ -69,7 +69,7 @@ def run(ortmi, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         if math.isinf(p):
             assert lp[r] == p
         else:
-            # fp32 rounding, and weights 2e-13 exact above units of 2^-44.
+            # fp32 rounding, and weights 2e-12 exact above units of 2^-44.
             assert abs(lp[r] - p) <= 2.0 ** -23 * abs(p) + 1e-9, (r, lp[r], p)
     return ids
 
