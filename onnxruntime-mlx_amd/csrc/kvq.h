@@ -46,11 +46,13 @@ struct Params {
     float *part, *ml;
     int ntile;                  // slabs: tiles of a sequence's columns
     int fused;                  // slabs: the tiles write the new rows themselves
+    int pieces;                 // new rows come in 16-byte pieces, rotated over the whole head
     int blk_shift;              // pages: log2(blk), or -1
-    int2* tiles;                // pages: (sequence, first column) of tiles of 64 columns
+    int2* tiles;                // pages: (sequence, first column) of prompt tiles
     int max_tiles;
     int* tile_count;
     int tile_chunk, tile_nsplit;  // pages: ranges of those tiles, at most nsplit of them
+    int paired;                   // slabs: two tiles a CU run at once
 };
 
 __device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {
@@ -131,64 +133,59 @@ __device__ __forceinline__ uint32_t encode_e4m3(double r) {
     return sign | (uint32_t)(((e + 7) << 3) + (int)rint(ldexp(a, 3 - e)) - 8);
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+// The stored code (int4: with its offset) of x / scale.
+__device__ __forceinline__ uint32_t encode(double x, float scale, int code) {
+    const double r = x / (double)scale;
+    if (code == kInt8) return (uint32_t)encode_int(r, -128, 127) & 0xFFu;
+    if (code == kFp8) return encode_e4m3(r);
+    return (uint32_t)(encode_int(r, -8, 7) + 8);
 }
 
-// One wave quantises one new row of one kv head and writes it to the cache.
+// One new row, key or value, of kv head h by 16 lanes (`lane` of them), two channels a step.
 template <bool PAGED>
 __device__ __forceinline__ void append_row(const Params& p, int b, const Seq& s, int r, int h,
-                                           bool is_v) {
-    const int lane = threadIdx.x & 63, hd = p.hd, pos = s.past + r;
+                                           bool is_v, int lane) {
+    const int hd = p.hd, pos = s.past + r;
     const int64_t row = cache_row<PAGED>(p, b, h, pos);
-    if (row < 0) return;
     const void* src = is_v ? p.v : p.k;
     const int64_t x0 = (int64_t)(s.tok0 + r) * p.kv_tok + (int64_t)h * hd;
     const void* w = is_v ? nullptr : p.kw;
     double rinv = 1.0;
-    if (w) {
+    if (p.kw) {  // (a value row's lanes go along)
         double ss = 0;
-        for (int c = lane; c < hd; c += 64) {
+        for (int c = lane; c < hd; c += 16) {
             const double x = load_elem(src, x0 + c, p.dtype);
             ss += x * x;
         }
-        rinv = 1.0 / sqrt(wave_sum64(ss) / hd + (double)p.eps);
+#pragma unroll
+        for (int o = 8; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        rinv = 1.0 / sqrt(ss / hd + (double)p.eps);
     }
-    auto elem = [&](int c) -> double {
-        double x = load_elem(src, x0 + c, p.dtype);
-        if (w) x = x * rinv * (double)load_elem(w, c, p.dtype);
-        return x;
-    };
+    if (row < 0) return;
     const bool rope = !is_v && p.cos;
     const int64_t prow = min((int64_t)pos, p.max_pos - 1) * p.half;
     const float* sc = is_v ? p.vs : p.ks;
     const bool chan = is_v ? p.v_chan : p.k_chan;
     uint8_t* dst = (is_v ? p.vc : p.kc) + row * row_bytes(p.code, hd);
-    for (int c0 = 2 * lane; c0 < hd; c0 += 128) {
-        double x[2] = {elem(c0), elem(c0 + 1)};
-        if (rope && c0 < 2 * p.half) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int c = c0 + i;
-                if (c >= 2 * p.half) break;  // odd `half`: the pair may end past the rotated part
-                const bool second = p.interleaved ? (c & 1) : c >= p.half;
-                const int f = p.interleaved ? c >> 1 : (second ? c - p.half : c);
-                const int other = p.interleaved ? c ^ 1 : (second ? c - p.half : c + p.half);
-                const double co = load_elem(p.cos, prow + f, p.dtype);
-                const double si = load_elem(p.sin, prow + f, p.dtype);
-                const double self = elem(c), part = elem(other);
-                x[i] = second ? self * co + part * si : self * co - part * si;
-            }
-        }
+    auto elem = [&](int c) -> double {
+        const double x = load_elem(src, x0 + c, p.dtype);
+        return w ? x * rinv * (double)load_elem(w, c, p.dtype) : x;
+    };
+    for (int c0 = 2 * lane; c0 < hd; c0 += 32) {
         uint32_t u[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const double r64 = x[i] / (double)sc[chan ? h * hd + c0 + i : 0];
-            if (p.code == kInt8) u[i] = (uint32_t)encode_int(r64, -128, 127) & 0xFFu;
-            else if (p.code == kInt4) u[i] = (uint32_t)(encode_int(r64, -8, 7) + 8);
-            else u[i] = encode_e4m3(r64);
+            const int c = c0 + i;
+            double x = elem(c);
+            if (rope && c < 2 * p.half) {
+                const bool second = p.interleaved ? (c & 1) : c >= p.half;
+                const int f = p.interleaved ? c >> 1 : (second ? c - p.half : c);
+                const double part = elem(p.interleaved ? c ^ 1 : (second ? c - p.half : c + p.half));
+                const double co = load_elem(p.cos, prow + f, p.dtype);
+                const double si = load_elem(p.sin, prow + f, p.dtype);
+                x = second ? x * co + part * si : x * co - part * si;
+            }
+            u[i] = encode(x, sc[chan ? h * hd + c : 0], p.code);
         }
         if (p.code == kInt4) {
             dst[c0 >> 1] = (uint8_t)(u[0] | (u[1] << 4));

@@ -8,70 +8,6 @@
 namespace ortmi {
 namespace kvq {
 
-// The last sequence that starts at or before token `tok`, and whether it has the token.
-__device__ __forceinline__ bool sequence_of_token(const Params& p, int tok, int& b, Seq& s) {
-    int lo = 0, hi = p.B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.cum[mid] <= tok) lo = mid;
-        else hi = mid;
-    }
-    b = lo;
-    s = sequence<true>(p, lo);
-    return tok >= s.tok0 && tok < s.tok0 + s.rows;
-}
-
-// The tiles of the sequences with more than 16 columns, in order, by one wave. Ranges
-// of tokens are clamped to the call's (sequence()), and at most max_tiles are written.
-__device__ void list_tiles(const Params& p) {
-    const int lane = threadIdx.x & 63, G = p.H / p.KV, w = page_width(p.dtype);
-    int base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int b = b0 + lane;
-        const int cols = b < p.B ? sequence<true>(p, b).rows * G : 0;
-        const int n = cols > 16 ? (cols + w - 1) / w : 0;
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += v;
-        }
-        const int first = base + incl - n;
-        for (int i = 0; i < n && first + i < p.max_tiles; ++i) p.tiles[first + i] = make_int2(b, w * i);
-        base += __shfl(incl, 63, 64);
-    }
-    if (lane == 0) *p.tile_count = min(base, p.max_tiles);
-}
-
-// New keys and values into the cache: one wave per (token, kv head, key or value). Pages: the
-// first workgroup lists the tiles.
-template <bool PAGED>
-__global__ __launch_bounds__(256) void append_kernel(Params p) {
-    int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if constexpr (PAGED) {
-        if (blockIdx.x == 0) {
-            if (threadIdx.x < 64 && p.tiles) list_tiles(p);
-            return;
-        }
-        item -= 4;
-    }
-    const int per = 2 * p.KV;
-    const int64_t tok = item / per;
-    if (tok >= p.T) return;
-    const int hv = (int)(item % per);
-    int b;
-    Seq s;
-    if constexpr (PAGED) {
-        if (!sequence_of_token(p, (int)tok, b, s)) return;
-    } else {
-        b = (int)(tok / p.S);
-        s = sequence<false>(p, b);
-    }
-    const int r = (int)tok - s.tok0;
-    if (r >= s.real) return;
-    append_row<PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV);
-}
-
 // Joins the ranges of the rows whose tile had more than one: a wave per (token, head).
 template <bool PAGED>
 __global__ __launch_bounds__(256) void merge_kernel(Params p) {
@@ -89,7 +25,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Params p) {
     }
     const int r = tok - s.tok0, cols = s.rows * G;
     if (r >= s.real) return;
-    const int w = PAGED ? (cols <= 16 ? 16 : page_width(p.dtype)) : tile_width(cols, p.dtype);
+    const int w = tile_width(cols, p.dtype);
     const int c0 = (r * G + head - h * G) / w * w;
     const int kend = s.keys_to((min(c0 + w, cols) - 1) / G, p.limit);
     const int chunk = PAGED && cols > 16 ? p.tile_chunk : p.chunk;
@@ -265,7 +201,7 @@ static void plan_slabs(int64_t B, int64_t S, int64_t H, int64_t KV, int64_t n, i
     const int64_t cols = S * (H / KV);
     const int w = tile_width((int)std::min<int64_t>(cols, 1 << 20), dtype);
     ntile = (int)((cols + w - 1) / w);
-    plan_ranges(B * KV * ntile, n, w == 16 ? 768 : 256, nsplit, chunk);
+    plan_ranges(B * KV * ntile, n, w == 16 ? 768 : 512, nsplit, chunk);
 }
 
 static void plan_pages(int64_t B, int64_t KV, int64_t n, int& nsplit, int& chunk) {
@@ -300,10 +236,14 @@ static int attend(Params& p, hipStream_t st) {
                        (!PAGED || (p.blk % 16 == 0 && p.nblk <= INT32_MAX / p.blk));
     if (!tiles) p.tiles = nullptr;
     p.fused = !PAGED && tiles && p.ntile == 1;
-    if (!p.fused) {
+    p.paired = p.B * p.KV * p.ntile <= 2 * device_cu_count();
+    for (const void* x : {p.k, p.v, p.cos, p.sin, p.kw}) bits |= reinterpret_cast<uintptr_t>(x);
+    p.pieces = tiles && (bits & 15) == 0 && (!p.cos || (2 * p.half == p.hd && !p.interleaved));
+    if (!p.fused && !p.pieces) {
         const int64_t items = (int64_t)p.T * 2 * p.KV;
-        hipLaunchKernelGGL((append_kernel<PAGED>), dim3((unsigned)((items + 3) / 4 + (PAGED ? 1 : 0))),
-                           dim3(256), 0, st, p);
+        hipLaunchKernelGGL((append_kernel<kInt8, 0, false, PAGED>),
+                           dim3((unsigned)((items + 15) / 16 + (PAGED ? 1 : 0))), dim3(256), 0, st,
+                           p);
         if (int rc = check_launch("kv append")) return rc;
     }
     if (!tiles) {
@@ -485,7 +425,7 @@ extern "C" size_t ortmi_paged_attention_quantized_workspace_size(
     int nsplit, chunk;
     kvq::plan_pages(batch, kv_num_heads, max_context, nsplit, chunk);
     return kvq::ranges_bytes(num_tokens * num_heads, nsplit, head_size) +
-           (size_t)(kvq::max_page_tiles(num_tokens, batch, num_heads / kv_num_heads, 32) + 1) * 8;
+           (size_t)(kvq::max_page_tiles(num_tokens, batch, num_heads / kv_num_heads, 64) + 1) * 8;
 }
 
 extern "C" int ortmi_paged_attention_quantized(
@@ -558,7 +498,7 @@ extern "C" int ortmi_paged_attention_quantized(
     if (kvq::tile_head(head_size)) {
         kvq::plan_pages(batch, kv_num_heads, max_context, p.nsplit, p.chunk);
         p.max_tiles = kvq::max_page_tiles(num_tokens, batch, num_heads / kv_num_heads,
-                                          kvq::page_width(dtype));
+                                          kvq::prompt_width(dtype));
         const size_t need = kvq::ranges_bytes(num_tokens * num_heads, p.nsplit, head_size) +
                             (size_t)(p.max_tiles + 1) * 8;
         if (!workspace || workspace_bytes < need)
@@ -568,7 +508,7 @@ extern "C" int ortmi_paged_attention_quantized(
         char* ws = kvq::place_ranges(p, static_cast<char*>(workspace));
         p.tile_count = reinterpret_cast<int*>(ws);
         p.tiles = reinterpret_cast<int2*>(ws + 8);
-        // Tiles of 64 columns: ranges of four times the keys (their work fills the GPU sooner).
+        // Prompt tiles: ranges of four times the keys (their work fills the GPU sooner).
         p.tile_chunk = (int)std::min<int64_t>(4LL * p.chunk, 1 << 23);
         p.tile_nsplit = (p.nsplit + 3) / 4;
     }

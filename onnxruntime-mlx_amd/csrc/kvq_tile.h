@@ -1,22 +1,30 @@
 // Attention over quantised key-value caches on the matrix cores (head sizes 64, 96, 128).
 //
-// A workgroup of 4 waves takes 16 NT columns, a column being one query row of one head of a
-// group (all heads of the group read the same keys), over a range of keys; its waves take
-// every fourth block of 32 keys and are joined at the end, ranges by merge_kernel. Scores are
-// computed transposed, S^T = K Q^T, with v_mfma_f32_16x16x32_f16: a lane then holds column
-// lane % 16 and, of a block's two key tiles, keys 4 (lane / 16) + i. That is already the order
-// in which the second product O^T = V^T P^T takes P as its right operand (the 8 keys of a
-// lane's k slots are those), so P never leaves its registers, and V is read with lane % 16
+// A column is one query row of one head of a group: all heads of a group read the same keys.
+// Scores are computed transposed, S^T = K Q^T, with v_mfma_f32_16x16x32_f16: a lane then holds
+// column lane % 16 and, of a tile of 16 keys, keys 4 (lane / 16) + i. Two tiles are already the
+// order in which the second product O^T = V^T P^T takes P as its right operand (the 8 keys of
+// a lane's k slots are those), so P never leaves its registers, and V is read with lane % 16
 // running over channels, 8 keys of a lane's own channels at a time, which byte permutes turn
-// into the left operand. Neither K nor V passes through LDS.
+// into the left operand.
 //
 // Codes are exact in fp16 (int8 and int4 by putting the byte under the exponent of 1024, fp8
 // by the conversion instruction). The key scales are folded into the query row, which is
 // rounded to fp16 after a power of two has brought its largest element to [2^10, 2^11): one
 // rounding of 2^-11 of an element, no range to leave. The probabilities are rounded to fp16
 // at up to 2^14 (2^6 where a row's running maximum is exact), 2^-11 of each and 2^-31 of the
-// largest at worst. fp32 tensors take both as two fp16 halves (22 bits) and twice the
-// products. Sums, maxima and outputs are fp32. The value scales are applied to the output.
+// largest at worst. Sums, maxima and outputs are fp32. The value scales are applied to the
+// output. Where few columns leave the matrix cores idle (token tiles), the query row is taken
+// as two fp16 halves, 22 bits; fp32 tensors take the probabilities as two halves too.
+//
+// Token tiles: 16 columns. A workgroup's 4 waves take every fourth block of 32 keys of its
+// range and are joined at the end; keys and values go from memory into registers, where each
+// wave decodes its own. Memory binds it: 4 sequences of 131072 int8 keys, 8 heads of 128, 190
+// us, 5.65 TB/s.
+//
+// Prompt tiles: 128 columns (fp32 64), 32 a wave, over blocks of 64 keys which the 4 waves
+// decode together into LDS, a quarter each, in the order that the products read: decoded once
+// for 128 columns. Two buffers, so that one barrier a block suffices, and two workgroups a CU.
 #pragma once
 
 #include "kvq.h"
@@ -28,13 +36,12 @@ namespace kvq {
 // grown by more than 2^kSlack: most blocks then rescale nothing.
 constexpr float kSlack = 8.f, kPBase = 6.f, kNone = -1e30f;
 
-// Columns of a tile for a sequence with `cols` columns in all. fp32 holds twice the query
-// registers: 64 columns of it do not fit.
+// Columns of a tile for a sequence with `cols` columns in all: 16, or those of a prompt tile
+// (fp32 holds twice the operands).
+__host__ __device__ constexpr int prompt_width(int dtype) { return dtype == ORTMI_F32 ? 64 : 128; }
 __host__ __device__ constexpr int tile_width(int cols, int dtype) {
-    return cols <= 16 ? 16 : (cols <= 32 || dtype == ORTMI_F32 ? 32 : 64);
+    return cols <= 16 ? 16 : prompt_width(dtype);
 }
-// Pages: of a sequence with more than 16.
-__host__ __device__ constexpr int page_width(int dtype) { return dtype == ORTMI_F32 ? 32 : 64; }
 
 __device__ __forceinline__ half2_t as_half2(uint32_t u) { return __builtin_bit_cast(half2_t, u); }
 
@@ -182,65 +189,72 @@ struct Source {
         vat = 4 * q * stride + m * L::kValStep;
         vat2 = 4 * q * stride + m * (L::kValStep / 2);
     }
-    // Slots of the two key tiles of block kb: -1 behind the end and where there is no block.
-    __device__ __forceinline__ int2 slots(int kb) const {
-        int s[2] = {-1, -1};
+    // Slot of the key tile at `key`: -1 behind the end and where there is no block.
+    __device__ __forceinline__ int slot(int key) const {
+        int s = -1;
+        if constexpr (PAGED) {
+            if (key < k1) {
+                const int lb = p.blk_shift >= 0 ? key >> p.blk_shift : key / p.blk;
+                const int id = lb < p.maxb ? p.bt[(int64_t)b * p.maxb + lb] : -1;
+                s = id >= 0 && id < p.nblk ? id * p.blk + (key - lb * p.blk) : -1;
+            }
+        }
+        return s;
+    }
+    // The resource of the cache rows of a tile in a page.
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t page(const uint8_t* base, int key, int slot) const {
+        const int rows = min(16, k1 - key);
+        const uint32_t bytes = slot < 0 ? 0u : (uint32_t)(rows - 1) * stride + L::RB;
+        return buffer_rsrc(base + (int64_t)max(slot, 0) * stride, bytes);
+    }
+    // A lane's share of the key tile at `key`.
+    __device__ __forceinline__ void keys(int key, int slot, uint32_t (&w)[L::KW]) const {
+        if constexpr (PAGED) {
+            L::load_key(page(kbase, key, slot), kat, kat2, w);
+        } else {
+            const uint32_t off = (uint32_t)(key - k0) * L::RB;
+            L::load_key(buffer_rsrc(kbase, (uint32_t)(k1 - k0) * L::RB), off + kat, off + kat2, w);
+        }
+    }
+    // Its 8 value rows of the two tiles at `key`.
+    __device__ __forceinline__ void values(int key, int slot0, int slot1, uint32_t (&w)[8][L::VW]) const {
         if constexpr (PAGED) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int key = kb + 16 * t;
-                if (key < k1) {
-                    const int lb = p.blk_shift >= 0 ? key >> p.blk_shift : key / p.blk;
-                    const int id = lb < p.maxb ? p.bt[(int64_t)b * p.maxb + lb] : -1;
-                    if (id >= 0 && id < p.nblk) s[t] = id * p.blk + (key - lb * p.blk);
-                }
-            }
-        }
-        return make_int2(s[0], s[1]);
-    }
-    __device__ __forceinline__ void load(int kb, int2 sl, Block<CODE, HD>& o) const {
-        if constexpr (!PAGED) {
-            const uint32_t bytes = (uint32_t)(k1 - k0) * L::RB;
-            const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(kbase, bytes);
-            const __amdgpu_buffer_rsrc_t vr = buffer_rsrc(vbase, bytes);
-            const uint32_t off = (uint32_t)(kb - k0) * L::RB;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                L::load_key(kr, off + kat + 16 * t * L::RB, off + kat2 + 16 * t * L::RB, o.k[t]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t r = ((j & 3) + 16 * (j >> 2)) * L::RB;
-                L::load_value(vr, off + vat + r, off + vat2 + r, o.v[j]);
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int slot = t ? sl.y : sl.x;
-                const int rows = min(16, k1 - kb - 16 * t);
-                const uint32_t bytes = slot < 0 ? 0u : (uint32_t)(rows - 1) * stride + L::RB;
-                const int64_t at = (int64_t)max(slot, 0) * stride;
-                const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(kbase + at, bytes);
-                const __amdgpu_buffer_rsrc_t vr = buffer_rsrc(vbase + at, bytes);
-                L::load_key(kr, kat, kat2, o.k[t]);
+                const __amdgpu_buffer_rsrc_t r = page(vbase, key + 16 * t, t ? slot1 : slot0);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    L::load_value(vr, vat + j * stride, vat2 + j * stride, o.v[4 * t + j]);
+                    L::load_value(r, vat + j * stride, vat2 + j * stride, w[4 * t + j]);
+            }
+        } else {
+            const uint32_t off = (uint32_t)(key - k0) * L::RB;
+            const __amdgpu_buffer_rsrc_t r = buffer_rsrc(vbase, (uint32_t)(k1 - k0) * L::RB);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t at = ((j & 3) + 16 * (j >> 2)) * L::RB;
+                L::load_value(r, off + vat + at, off + vat2 + at, w[j]);
             }
         }
+    }
+    __device__ __forceinline__ int2 slots(int kb) const { return make_int2(slot(kb), slot(kb + 16)); }
+    __device__ __forceinline__ void load(int kb, int2 sl, Block<CODE, HD>& o) const {
+        keys(kb, sl.x, o.k[0]);
+        keys(kb + 16, sl.y, o.k[1]);
+        values(kb, sl.x, sl.y, o.v);
     }
 };
 
-template <int HD, int NT, bool F32>
-struct TileShared {
-    static constexpr int kCols = 16 * NT;
-    static constexpr int kRow = HD + 4;  // floats of a row, four more than a multiple of the banks
-    // Raw query rows and their cos/sin; then two waves' outputs; then the tile's output rows.
-    static constexpr int kFloats = 2 * kCols * kRow;
-    __align__(16) float rows[kFloats];
-    __align__(16) half_t q[(F32 ? 2 : 1) * kCols * HD];
-    float f[kCols], inv[kCols];
-    int pos[kCols];
-    float m[4][kCols], l[4][kCols];
+constexpr int kPass = 2;  // groups of 16 columns whose queries are staged at once
+template <int HD>
+constexpr int kRowFloats = HD + 4;  // of a row in LDS: four more than a multiple of the banks
+
+// Queries of 16 NC columns, their halves (where split), factors and positions.
+template <int HD, int NC, bool SPLIT>
+struct Queries {
+    static constexpr int kCols = 16 * NC, kStage = NC < kPass ? NC : kPass;
+    // Rows of a pass and their cos/sin.
+    __align__(16) float rows[2 * 16 * kStage * kRowFloats<HD>];
+    __align__(16) half_t q[(SPLIT ? 2 : 1) * kCols * HD];
 };
 
 // N consecutive elements of a 16-byte aligned row as fp32.
@@ -276,44 +290,42 @@ __device__ __forceinline__ float load_one(const void* base, int64_t at, int dtyp
     return dtype == ORTMI_F16 ? (float)__builtin_bit_cast(half_t, u) : to_f32(u);
 }
 
-// The query rows of columns c0 .. c0 + 16 NT - 1 into LDS, 16 lanes a column: (normalised and)
+// The query rows of columns c0 .. c0 + 16 NC - 1 into LDS, 16 lanes a column: (normalised and)
 // rotated, times the key scales, brought to [2^10, 2^11) and rounded to fp16, in the order
-// [column][k step][quarter][8] of the right operand (fp32: the second halves behind).
-template <int CODE, int HD, int NT, bool F32>
+// [column][k step][quarter][8] of the right operand (the second halves behind). f: what a
+// product is to be multiplied by; pos: the column's position, -1 for none.
+template <int CODE, int HD, int NC, bool F32, bool SPLIT>
 __device__ __forceinline__ void stage_queries(const Params& p, const Seq& s, int h, int c0,
-                                              TileShared<HD, NT, F32>& sh) {
+                                              Queries<HD, NC, SPLIT>& sh, float* f, int* pos) {
     using L = Layout<CODE, HD>;
-    using SH = TileShared<HD, NT, F32>;
-    constexpr int N = HD / 16;
-    const int G = p.H / p.KV, tid = threadIdx.x, lane = tid & 15;
-    float x[NT][N];
+    using SH = Queries<HD, NC, SPLIT>;
+    constexpr int N = HD / 16, R = kRowFloats<HD>, F = HD / 32;
+    const int G = p.H / p.KV, tid = threadIdx.x, lane = tid & 15, group = tid >> 4;
     const bool rope = p.cos != nullptr;
+    float x[NC][N], cs[NC][2 * F];
 #pragma unroll
-    for (int cc = 0; cc < NT; ++cc) {
-        const int c = 16 * cc + (tid >> 4), r = (c0 + c) / G, g = (c0 + c) - r * G;
+    for (int cc = 0; cc < NC; ++cc) {
+        const int c = 16 * cc + group, r = (c0 + c) / G, g = (c0 + c) - r * G;
         const bool live = r < s.real;
-        const int tok = s.tok0 + (live ? r : 0), pos = s.past + (live ? r : 0);
+        const int tok = s.tok0 + (live ? r : 0), at = s.past + (live ? r : 0);
         load_piece<N, F32>(p.q, (int64_t)tok * p.q_tok + (int64_t)(h * G + g) * HD + lane * N,
                            p.dtype, x[cc]);
         if (rope) {
-            const int64_t prow = min((int64_t)pos, p.max_pos - 1) * p.half;
-            float* cs = sh.rows + (SH::kCols + c) * SH::kRow;
+            const int64_t prow = min((int64_t)at, p.max_pos - 1) * p.half;
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-                const int f = lane + 16 * i;
-                if (f < p.half) {
-                    cs[2 * f] = load_one<F32>(p.cos, prow + f, p.dtype);
-                    cs[2 * f + 1] = load_one<F32>(p.sin, prow + f, p.dtype);
-                }
+            for (int i = 0; i < F; ++i) {
+                const int64_t k = prow + min(lane + 16 * i, p.half - 1);
+                cs[cc][2 * i] = load_one<F32>(p.cos, k, p.dtype);
+                cs[cc][2 * i + 1] = load_one<F32>(p.sin, k, p.dtype);
             }
         }
-        if (lane == 0) sh.pos[c] = live ? pos : -1;
+        if (lane == 0) pos[c] = live ? at : -1;
     }
     if (p.qw) {
         float w[N];
         load_piece<N, F32>(p.qw, lane * N, p.dtype, w);
 #pragma unroll
-        for (int cc = 0; cc < NT; ++cc) {
+        for (int cc = 0; cc < NC; ++cc) {
             float ss = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i) ss += x[cc][i] * x[cc][i];
@@ -322,13 +334,6 @@ __device__ __forceinline__ void stage_queries(const Params& p, const Seq& s, int
             for (int i = 0; i < N; ++i) x[cc][i] = x[cc][i] * rinv * w[i];
         }
     }
-#pragma unroll
-    for (int cc = 0; cc < NT; ++cc) {
-        float* row = sh.rows + (16 * cc + (tid >> 4)) * SH::kRow + lane * N;
-#pragma unroll
-        for (int i = 0; i < N; ++i) row[i] = x[cc][i];
-    }
-    __syncthreads();
     // Element e of a column is channel ch[e]; the channels and scales serve every column.
     int ch[N];
     float sc[N];
@@ -339,38 +344,56 @@ __device__ __forceinline__ void stage_queries(const Params& p, const Seq& s, int
         sc[i] = p.ks[p.k_chan ? h * HD + ch[i] : 0];
     }
 #pragma unroll
-    for (int cc = 0; cc < NT; ++cc) {
-        const int c = 16 * cc + (tid >> 4);
-        const float* row = sh.rows + c * SH::kRow;
-        const float* cs = sh.rows + (SH::kCols + c) * SH::kRow;
-        float y[N], top = 0.f;
+    for (int c1 = 0; c1 < NC; c1 += SH::kStage) {
+        if (c1) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int k = ch[i];
-            float v = row[k];
-            if (rope && k < 2 * p.half) {
-                const bool second = p.interleaved ? (k & 1) : k >= p.half;
-                const int f = p.interleaved ? k >> 1 : (second ? k - p.half : k);
-                const float o = row[p.interleaved ? k ^ 1 : (second ? k - p.half : k + p.half)];
-                const float co = cs[2 * f], si = cs[2 * f + 1];
-                v = second ? v * co + o * si : v * co - o * si;
+        for (int cc = 0; cc < SH::kStage; ++cc) {
+            float* row = sh.rows + (16 * cc + group) * R;
+            float* turn = sh.rows + (16 * (SH::kStage + cc) + group) * R;
+#pragma unroll
+            for (int i = 0; i < N; ++i) row[lane * N + i] = x[c1 + cc][i];
+#pragma unroll
+            for (int i = 0; i < F; ++i) {
+                turn[2 * (lane + 16 * i)] = cs[c1 + cc][2 * i];
+                turn[2 * (lane + 16 * i) + 1] = cs[c1 + cc][2 * i + 1];
             }
-            y[i] = v * sc[i];
-            top = fmaxf(top, fabsf(y[i]));
         }
-        top = group_max<16>(top);
-        // A row of zeros, or with an infinity, is taken as it is.
-        const int ex = top > 0.f && top < INFINITY ? max(-100, min(ilogbf(top), 116)) : 10;
-        const bool live = sh.pos[c] >= 0;
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float z = live ? ldexpf(y[i], 10 - ex) : 0.f;
-            const half_t hi = (half_t)z;
-            sh.q[c * HD + lane * N + i] = hi;
-            if constexpr (F32) sh.q[(16 * NT + c) * HD + lane * N + i] = (half_t)(z - (float)hi);
+        for (int cc = 0; cc < SH::kStage; ++cc) {
+            const int c = 16 * (c1 + cc) + group;
+            const float* row = sh.rows + (16 * cc + group) * R;
+            const float* turn = sh.rows + (16 * (SH::kStage + cc) + group) * R;
+            float y[N], top = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int k = ch[i];
+                float v = row[k];
+                if (rope && k < 2 * p.half) {
+                    const bool second = p.interleaved ? (k & 1) : k >= p.half;
+                    const int t = p.interleaved ? k >> 1 : (second ? k - p.half : k);
+                    const float o = row[p.interleaved ? k ^ 1 : (second ? k - p.half : k + p.half)];
+                    v = second ? v * turn[2 * t] + o * turn[2 * t + 1]
+                               : v * turn[2 * t] - o * turn[2 * t + 1];
+                }
+                y[i] = v * sc[i];
+                top = fmaxf(top, fabsf(y[i]));
+            }
+            top = group_max<16>(top);
+            // A row of zeros, or with an infinity, is taken as it is.
+            const int ex = top > 0.f && top < INFINITY ? max(-100, min(ilogbf(top), 116)) : 10;
+            const bool live = pos[c] >= 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float z = live ? ldexpf(y[i], 10 - ex) : 0.f;
+                const half_t hi = (half_t)z;
+                sh.q[c * HD + lane * N + i] = hi;
+                if constexpr (SPLIT) sh.q[(SH::kCols + c) * HD + lane * N + i] = (half_t)(z - (float)hi);
+            }
+            if (lane == 0) f[c] = ldexpf(p.scale, ex - 10);
         }
-        if (lane == 0) sh.f[c] = ldexpf(p.scale, ex - 10);
     }
+    __syncthreads();
 }
 
 __device__ __forceinline__ half8_t pack_p(const float (&a)[4], const float (&b)[4]) {
@@ -383,35 +406,328 @@ __device__ __forceinline__ half8_t pack_p(const float (&a)[4], const float (&b)[
     return r;
 }
 
-// One tile of columns c0 .. over keys [k0, k1) of sequence s: range `split` of `nsplit`.
-template <int CODE, int HD, int NT, bool F32, bool PAGED>
-__device__ __forceinline__ void attend_tile(const Params& p, const Seq& s, int b, int h, int c0,
-                                            int k0, int k1, int split, int nsplit,
-                                            TileShared<HD, NT, F32>& sh) {
+// Scores of the lane's 4 keys of a tile at `key` for a column at position pos, in units of
+// log2(e): -inf where the column does not attend the key (later ones, behind the end, no page).
+__device__ __forceinline__ void mask_scores(float (&x)[4], int key, int end) {
+    const int q = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = key + 4 * q + i > end ? -INFINITY : x[i];
+}
+
+// exp2 of the scores about the column's reference, rounded to fp16 as the second product's
+// operand (and, SPLIT, what the rounding left), added to the lane's sum.
+template <bool SPLIT>
+__device__ __forceinline__ void probabilities(const float (&x0)[4], const float (&x1)[4], float m,
+                                              float& l, half8_t& p, half8_t& rest) {
+    const float ref = m - kPBase;
+    float a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a[i] = __builtin_amdgcn_exp2f(x0[i] - ref);
+        b[i] = __builtin_amdgcn_exp2f(x1[i] - ref);
+        l += a[i] + b[i];
+    }
+    p = pack_p(a, b);
+    if constexpr (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] -= (float)p[i];
+            b[i] -= (float)p[4 + i];
+        }
+        rest = pack_p(a, b);
+    }
+}
+
+__device__ __forceinline__ float max4(const float (&x)[4]) {
+    return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+}
+// Maximum and sum over the four quarters that share a column.
+__device__ __forceinline__ float quarters_max(float v) {
+    LanePair pr = swap16(v);
+    pr = swap32(fmaxf(pr.a, pr.b));
+    return fmaxf(pr.a, pr.b);
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+    LanePair pr = swap16(v);
+    pr = swap32(pr.a + pr.b);
+    return pr.a + pr.b;
+}
+
+#define ORTMI_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
+
+// What a column's output is multiplied by, from its maximum and sum and the sink of its head.
+template <bool F32, bool PAGED>
+__device__ __forceinline__ float output_factor(const Params& p, int head, float m, float l) {
+    float a = 1.f;
+    if (PAGED && p.sink) {
+        const float sk = load_one<F32>(p.sink, head, p.dtype) * 1.44269504088896341f;
+        const float mm = fmaxf(m, sk);
+        a = __builtin_amdgcn_exp2f(m - mm);
+        l = l * a + __builtin_amdgcn_exp2f(sk - mm + kPBase);
+    }
+    return l != 0.f ? a / l : 0.f;
+}
+
+// N (4 or 8) neighbouring channels of an output row; a factor of 0 gives zeros whatever they are.
+template <int N, int HD, bool F32>
+__device__ __forceinline__ void store_piece(const Params& p, int64_t row, int h, int ch,
+                                            const float (&v)[N], float inv) {
+    float y[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        y[j] = inv != 0.f ? v[j] * inv * p.vs[p.v_chan ? h * HD + ch + j : 0] : 0.f;
+    if constexpr (F32) {
+        float* o = static_cast<float*>(p.out) + row * HD + ch;
+#pragma unroll
+        for (int j = 0; j < N; j += 2) *reinterpret_cast<float2*>(o + j) = make_float2(y[j], y[j + 1]);
+    } else {
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            const uint16_t a = p.dtype == ORTMI_F16 ? __builtin_bit_cast(uint16_t, (half_t)y[2 * j])
+                                                    : from_f32<uint16_t>(y[2 * j]);
+            const uint16_t b = p.dtype == ORTMI_F16 ? __builtin_bit_cast(uint16_t, (half_t)y[2 * j + 1])
+                                                    : from_f32<uint16_t>(y[2 * j + 1]);
+            w[j] = a | ((uint32_t)b << 16);
+        }
+        uint16_t* o = static_cast<uint16_t*>(p.out) + row * HD + ch;
+        if constexpr (N == 8) *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (N == 4) *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(o) = w[0];
+    }
+}
+
+// ----------------------------------------------------------------- token tiles --
+template <int HD, bool F32>
+struct TokenShared {
+    union {
+        Queries<HD, 1, true> queries;
+        __align__(16) float4_t out[2][HD / 16][64];    // two waves' outputs
+        __align__(16) float rows[16 * kRowFloats<HD>];  // the tile's output
+    };
+    float f[16], inv[16];
+    int pos[16];
+    float m[4][16], l[4][16];
+};
+
+// One tile of columns 0 .. 15 over keys [k0, k1) of sequence s: range `split` of `nsplit`.
+template <int CODE, int HD, bool F32, bool PAGED>
+__device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b, int h, int k0,
+                                           int k1, int split, int nsplit, TokenShared<HD, F32>& sh) {
     using L = Layout<CODE, HD>;
-    using SH = TileShared<HD, NT, F32>;
     constexpr int KS = L::KS, MT = L::MT;
     const int lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
     const int wave = uniform(threadIdx.x >> 6);
     const int G = p.H / p.KV;
 
-    stage_queries<CODE, HD, NT, F32>(p, s, h, c0, sh);
+    // The first block's rows are on their way while the queries are staged.
+    const Source<CODE, HD, PAGED> src(p, b, h, k0, k1);
+    int kb = k0 + 32 * wave;
+    int2 sl = src.slots(kb), sl_n = src.slots(kb + 128);
+    Block<CODE, HD> cur, nxt;
+    if (kb < k1) src.load(kb, sl, cur);
+    stage_queries<CODE, HD, 1, F32, true>(p, s, h, 0, sh.queries, sh.f, sh.pos);
+    const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries.q);
+    half8_t Q[KS], QL[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        Q[ks] = sq[(n * KS + ks) * 4 + q];
+        QL[ks] = sq[((16 + n) * KS + ks) * 4 + q];
+    }
+    const float f = sh.f[n];
+    const int pos = sh.pos[n];
+    const int first = s.past;  // the lowest position of the tile
+
+    float4_t O[MT];
+    float m = kNone, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < MT; ++d) O[d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (; kb < k1; kb += 128) {
+        const int2 sl_c = sl;
+        if (kb + 128 < k1) {
+            src.load(kb + 128, sl_n, nxt);
+            sl = sl_n;
+            sl_n = src.slots(kb + 256);
+        }
+        float x[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float4_t S{0.f, 0.f, 0.f, 0.f}, SL{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const half8_t a = L::key_step(cur.k[t], ks);
+                S = ORTMI_MFMA(a, Q[ks], S);
+                SL = ORTMI_MFMA(a, QL[ks], SL);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t][i] = (S[i] + SL[i]) * f;
+        }
+        if (kb + 31 > first || kb + 32 > k1 || (PAGED && (sl_c.x < 0 || sl_c.y < 0))) {
+            const int end = min(pos, k1 - 1);
+            mask_scores(x[0], kb, PAGED && sl_c.x < 0 ? -1 : end);
+            mask_scores(x[1], kb + 16, PAGED && sl_c.y < 0 ? -1 : end);
+        }
+        const float top = fmaxf(max4(x[0]), max4(x[1]));
+        if (__any(top > m + kSlack)) {
+            const float mm = fmaxf(m, quarters_max(fmaxf(top, kNone)));
+            const float a = __builtin_amdgcn_exp2f(m - mm);
+            m = mm;
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < MT; ++d) O[d] *= a;
+        }
+        half8_t P, PL;
+        probabilities<F32>(x[0], x[1], m, l, P, PL);
+#pragma unroll
+        for (int u = 0; u < MT / 2; ++u) {
+            half8_t a[2];
+            L::value_steps(cur.v, u, a[0], a[1]);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                O[2 * u + d] = ORTMI_MFMA(a[d], P, O[2 * u + d]);
+                if constexpr (F32) O[2 * u + d] = ORTMI_MFMA(a[d], PL, O[2 * u + d]);
+            }
+        }
+        cur = nxt;
+    }
+
+    // The four waves: maxima and sums, then outputs in two steps through LDS.
+    l = quarters_sum(l);
+    if (q == 0) {
+        sh.m[wave][n] = m;
+        sh.l[wave][n] = l;
+    }
     __syncthreads();
-    const half8_t* sq = reinterpret_cast<const half8_t*>(sh.q);
+    float mm = kNone, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sh.m[w][n]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum += sh.l[w][n] * __builtin_amdgcn_exp2f(sh.m[w][n] - mm);
+    const float a = __builtin_amdgcn_exp2f(m - mm);
+#pragma unroll
+    for (int d = 0; d < MT; ++d) O[d] *= a;
+#pragma unroll
+    for (int step = 2; step; step >>= 1) {
+        if (wave >= step && wave < 2 * step) {
+#pragma unroll
+            for (int d = 0; d < MT; ++d) sh.out[wave - step][d][lane] = O[d];
+        }
+        __syncthreads();
+        if (wave < step) {
+#pragma unroll
+            for (int d = 0; d < MT; ++d) O[d] += sh.out[wave][d][lane];
+        }
+        __syncthreads();
+    }
+    // Output rows by all waves. A partial row stays unscaled, with its maximum and sum.
+    if (wave == 0) {
+        float* row = sh.rows + n * kRowFloats<HD>;
+#pragma unroll
+        for (int d = 0; d < MT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) row[L::value_channel(4 * q + i, d)] = O[d][i];
+        const int r = n / G, head = h * G + (n - r * G);
+        if (q == 0 && r < s.real) {
+            const int64_t orow = (int64_t)(s.tok0 + r) * p.H + head;
+            if (nsplit > 1) {
+                p.ml[(orow * p.nsplit + split) * 2] = mm;
+                p.ml[(orow * p.nsplit + split) * 2 + 1] = sum;
+            } else {
+                sh.inv[n] = output_factor<F32, PAGED>(p, head, mm, sum);
+            }
+        }
+    }
+    __syncthreads();
+    constexpr int kPieces = HD / 4;  // of a row: four channels a thread and step
+    for (int i = threadIdx.x; i < 16 * kPieces; i += 256) {
+        const int c = i / kPieces, ch = 4 * (i % kPieces), r = c / G;
+        if (r >= s.rows) break;
+        const int64_t orow = (int64_t)(s.tok0 + r) * p.H + h * G + (c - r * G);
+        const float4_t v = *reinterpret_cast<const float4_t*>(sh.rows + c * kRowFloats<HD> + ch);
+        if (nsplit > 1 && r < s.real) {
+            *reinterpret_cast<float4_t*>(p.part + (orow * p.nsplit + split) * HD + ch) = v;
+        } else if (nsplit <= 1 || split == 0) {
+            const float y[4] = {v[0], v[1], v[2], v[3]};
+            store_piece<4, HD, F32>(p, orow, h, ch, y, r < s.real ? sh.inv[c] : 0.f);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- prompt tiles --
+template <int CODE, int HD, bool F32>
+struct PromptShared {
+    static constexpr int kNT = F32 ? 1 : 2, kCols = 64 * kNT;
+    union {
+        Queries<HD, 4 * kNT, F32> queries;
+        struct {  // two blocks of 64 keys: [key tile][k step], [half][channel tile], by lane
+            half8_t k[2][4][HD / 32][64], v[2][2][HD / 16][64];
+        };
+    };
+    float f[kCols];
+    int pos[kCols];
+};
+
+// One tile of columns c0 .. over keys [k0, k1) of sequence s: range `split` of `nsplit`.
+template <int CODE, int HD, bool F32, bool PAGED>
+__device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b, int h, int c0,
+                                            int k0, int k1, int split, int nsplit,
+                                            PromptShared<CODE, HD, F32>& sh) {
+    using L = Layout<CODE, HD>;
+    using SH = PromptShared<CODE, HD, F32>;
+    constexpr int KS = L::KS, MT = L::MT, NT = SH::kNT, UH = (MT / 2 + 1) / 2;
+    const int lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+    const int wave = uniform(threadIdx.x >> 6);
+    const int G = p.H / p.KV;
+    const Source<CODE, HD, PAGED> src(p, b, h, k0, k1);
+
+    // Of a block at kb a wave decodes key tile `wave`, and of the values of its half of the
+    // keys (wave / 2) half of the channel tiles.
+    uint32_t rk[L::KW], rv[8][L::VW];
+    int slot[4], slot_n[4];
+    auto slots = [&](int kb, int (&sl)[4]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sl[t] = src.slot(kb + 16 * t);
+    };
+    auto load = [&](int kb, const int (&sl)[4]) {
+        const int k = wave & 1 ? (wave & 2 ? sl[3] : sl[1]) : (wave & 2 ? sl[2] : sl[0]);
+        src.keys(kb + 16 * wave, k, rk);
+        src.values(kb + 32 * (wave >> 1), wave & 2 ? sl[2] : sl[0], wave & 2 ? sl[3] : sl[1], rv);
+    };
+    auto decode = [&](int buf) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) sh.k[buf][wave][ks][lane] = L::key_step(rk, ks);
+#pragma unroll
+        for (int u = 0; u < MT / 2; ++u)
+            if ((u < UH) == !(wave & 1)) {
+                half8_t a, c;
+                L::value_steps(rv, u, a, c);
+                sh.v[buf][wave >> 1][2 * u][lane] = a;
+                sh.v[buf][wave >> 1][2 * u + 1][lane] = c;
+            }
+    };
+
+    slots(k0, slot);
+    load(k0, slot);
+    stage_queries<CODE, HD, 4 * NT, F32, F32>(p, s, h, c0, sh.queries, sh.f, sh.pos);
+    const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries.q);
     half8_t Q[NT][KS], QL[F32 ? NT : 1][KS];
     float f[NT];
     int pos[NT];
+    const int cw = 16 * NT * wave;  // the wave's columns
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            Q[t][ks] = sq[((16 * t + n) * KS + ks) * 4 + q];
-            if constexpr (F32) QL[t][ks] = sq[((16 * (NT + t) + n) * KS + ks) * 4 + q];
+            Q[t][ks] = sq[((cw + 16 * t + n) * KS + ks) * 4 + q];
+            if constexpr (F32) QL[t][ks] = sq[((SH::kCols + cw + 16 * t + n) * KS + ks) * 4 + q];
         }
-        f[t] = sh.f[16 * t + n];
-        pos[t] = sh.pos[16 * t + n];
+        f[t] = sh.f[cw + 16 * t + n];
+        pos[t] = sh.pos[cw + 16 * t + n];
     }
-    const int first = s.past + c0 / G;  // the lowest position of the tile
+    // The lowest and the highest position of the wave's columns (none: the latter is -1).
+    const int first = s.past + (c0 + cw) / G;
+    const int last = (c0 + cw) / G < s.real
+                         ? s.past + min((c0 + cw + 16 * NT - 1) / G, s.real - 1) : -1;
 
     float4_t O[MT][NT];
     float m[NT], l[NT];
@@ -422,219 +738,271 @@ __device__ __forceinline__ void attend_tile(const Params& p, const Seq& s, int b
 #pragma unroll
         for (int d = 0; d < MT; ++d) O[d][t] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-
-    const Source<CODE, HD, PAGED> src(p, b, h, k0, k1);
-    int kb = k0 + 32 * wave;
-    int2 sl = src.slots(kb), sl_n = src.slots(kb + 128);
-    Block<CODE, HD> cur, nxt;
-    if (kb < k1) src.load(kb, sl, cur);
-    for (; kb < k1; kb += 128) {
-        const int2 sl_c = sl;
-        if (kb + 128 < k1) {
-            src.load(kb + 128, sl_n, nxt);
-            sl = sl_n;
-            sl_n = src.slots(kb + 256);
+    __syncthreads();  // the queries are read: the blocks take their place
+    decode(0);
+    slots(k0 + 64, slot_n);
+    if (k0 + 64 < k1) load(k0 + 64, slot_n);
+    __syncthreads();
+    int buf = 0;
+    for (int kb = k0; kb < k1; kb += 64, buf ^= 1) {
+        const int sl[4] = {slot[0], slot[1], slot[2], slot[3]};
+        if (kb + 64 < k1) {
+            decode(buf ^ 1);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) slot[t] = slot_n[t];
+            slots(kb + 128, slot_n);
+            if (kb + 128 < k1) load(kb + 128, slot_n);
         }
-        float4_t S[2][NT];
+        if (kb <= last) {
+            float x[NT][4][4];
 #pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2) {
+            for (int t4 = 0; t4 < 4; ++t4) {
+                float4_t S[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) S[t2][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < NT; ++t) S[t] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const half8_t a = L::key_step(cur.k[t2], ks);
+                for (int ks = 0; ks < KS; ++ks) {
+                    const half8_t a = sh.k[buf][t4][ks][lane];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    S[t2][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, Q[t][ks], S[t2][t], 0, 0, 0);
-                    if constexpr (F32)
-                        S[t2][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, QL[t][ks], S[t2][t], 0, 0, 0);
+                    for (int t = 0; t < NT; ++t) {
+                        S[t] = ORTMI_MFMA(a, Q[t][ks], S[t]);
+                        if constexpr (F32) S[t] = ORTMI_MFMA(a, QL[t][ks], S[t]);
+                    }
                 }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[t][t4][i] = S[t][i] * f[t];
             }
-        }
-        // Keys that a column does not attend: later ones, behind the end, of no page.
-        const bool masked = kb + 31 > first || kb + 32 > k1 ||
-                            (PAGED && (sl_c.x < 0 || sl_c.y < 0));
-        float x[NT][2][4];
-        bool grow = false;
+            const bool gone = PAGED && (sl[0] < 0 || sl[1] < 0 || sl[2] < 0 || sl[3] < 0);
+            if (kb + 63 > first || kb + 64 > k1 || gone) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[t][t2][i] = S[t2][t][i] * f[t];
-            if (masked) {
-#pragma unroll
-                for (int t2 = 0; t2 < 2; ++t2) {
-                    const bool none = PAGED && (t2 ? sl_c.y : sl_c.x) < 0;
-                    const int end = none ? -1 : min(pos[t], k1 - 1);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[t][t2][i] = kb + 16 * t2 + 4 * q + i > end ? -INFINITY : x[t][t2][i];
-                }
+                    for (int t4 = 0; t4 < 4; ++t4)
+                        mask_scores(x[t][t4], kb + 16 * t4,
+                                    PAGED && sl[t4] < 0 ? -1 : min(pos[t], k1 - 1));
             }
-            const float top =
-                fmaxf(fmaxf(fmaxf(x[t][0][0], x[t][0][1]), fmaxf(x[t][0][2], x[t][0][3])),
-                      fmaxf(fmaxf(x[t][1][0], x[t][1][1]), fmaxf(x[t][1][2], x[t][1][3])));
-            grow |= top > m[t] + kSlack;
-        }
-        if (__any(grow)) {
+            bool grow = false;
+            float top[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float top = kNone;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(x[t][0][i], x[t][1][i]));
-                LanePair pr = swap16(top);
-                pr = swap32(fmaxf(pr.a, pr.b));
-                const float mm = fmaxf(m[t], fmaxf(pr.a, pr.b));
-                const float a = __builtin_amdgcn_exp2f(m[t] - mm);
-                m[t] = mm;
-                l[t] *= a;
-#pragma unroll
-                for (int d = 0; d < MT; ++d) O[d][t] *= a;
+                top[t] = fmaxf(fmaxf(max4(x[t][0]), max4(x[t][1])), fmaxf(max4(x[t][2]), max4(x[t][3])));
+                grow |= top[t] > m[t] + kSlack;
             }
-        }
-        half8_t P[NT], PL[F32 ? NT : 1];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const float ref = m[t] - kPBase;
-            float e[2][4];
-#pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[t2][i] = __builtin_amdgcn_exp2f(x[t][t2][i] - ref);
-                    l[t] += e[t2][i];
-                }
-            P[t] = pack_p(e[0], e[1]);
-            if constexpr (F32) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[0][i] -= (float)P[t][i];
-                    e[1][i] -= (float)P[t][4 + i];
-                }
-                PL[t] = pack_p(e[0], e[1]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < MT / 2; ++u) {
-            half8_t a[2];
-            L::value_steps(cur.v, u, a[0], a[1]);
-#pragma unroll
-            for (int d = 0; d < 2; ++d)
+            if (__any(grow)) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    float4_t& o = O[2 * u + d][t];
-                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[d], P[t], o, 0, 0, 0);
-                    if constexpr (F32)
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[d], PL[t], o, 0, 0, 0);
+                    const float mm = fmaxf(m[t], quarters_max(fmaxf(top[t], kNone)));
+                    const float a = __builtin_amdgcn_exp2f(m[t] - mm);
+                    m[t] = mm;
+                    l[t] *= a;
+#pragma unroll
+                    for (int d = 0; d < MT; ++d) O[d][t] *= a;
                 }
-        }
-        cur = nxt;
-    }
-
-    // The four waves: maxima and sums, then outputs in two steps through LDS.
+            }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        LanePair pr = swap16(l[t]);
-        pr = swap32(pr.a + pr.b);
-        l[t] = pr.a + pr.b;
-        if (q == 0) {
-            sh.m[wave][16 * t + n] = m[t];
-            sh.l[wave][16 * t + n] = l[t];
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        float mm = kNone, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sh.m[w][16 * t + n]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-            sum += sh.l[w][16 * t + n] * __builtin_amdgcn_exp2f(sh.m[w][16 * t + n] - mm);
-        const float a = __builtin_amdgcn_exp2f(m[t] - mm);
-#pragma unroll
-        for (int d = 0; d < MT; ++d) O[d][t] *= a;
-        m[t] = mm;
-        l[t] = sum;
-    }
-    float4_t* so = reinterpret_cast<float4_t*>(sh.rows);
-    constexpr int kSlotVecs = MT * NT * 64;
-#pragma unroll
-    for (int step = 2; step; step >>= 1) {
-        if (wave >= step && wave < 2 * step) {
-#pragma unroll
-            for (int d = 0; d < MT; ++d)
+            for (int j = 0; j < 2; ++j) {
+                half8_t P[NT], PL[NT];
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
-                    so[(wave - step) * kSlotVecs + (d * NT + t) * 64 + lane] = O[d][t];
-        }
-        __syncthreads();
-        if (wave < step) {
+                    probabilities<F32>(x[t][2 * j], x[t][2 * j + 1], m[t], l[t], P[t], PL[t]);
 #pragma unroll
-            for (int d = 0; d < MT; ++d)
+                for (int d = 0; d < MT; ++d) {
+                    const half8_t a = sh.v[buf][j][d][lane];
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    O[d][t] += so[wave * kSlotVecs + (d * NT + t) * 64 + lane];
-        }
-        __syncthreads();
-    }
-    // Output rows by all waves. A partial row stays unscaled, with its maximum and sum.
-    if (wave == 0) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float* row = sh.rows + (16 * t + n) * SH::kRow;
-#pragma unroll
-            for (int d = 0; d < MT; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) row[L::value_channel(4 * q + i, d)] = O[d][t][i];
-            const int c = c0 + 16 * t + n, r = c / G, head = h * G + (c - r * G);
-            if (q == 0 && r < s.real) {
-                const int64_t orow = (int64_t)(s.tok0 + r) * p.H + head;
-                if (nsplit > 1) {
-                    p.ml[(orow * p.nsplit + split) * 2] = m[t];
-                    p.ml[(orow * p.nsplit + split) * 2 + 1] = l[t];
-                } else {
-                    float a = 1.f, sum = l[t];
-                    if (PAGED && p.sink) {
-                        const float sk = load_one<F32>(p.sink, head, p.dtype) * 1.44269504088896341f;
-                        const float mm = fmaxf(m[t], sk);
-                        a = __builtin_amdgcn_exp2f(m[t] - mm);
-                        sum = sum * a + __builtin_amdgcn_exp2f(sk - mm + kPBase);
+                    for (int t = 0; t < NT; ++t) {
+                        O[d][t] = ORTMI_MFMA(a, P[t], O[d][t]);
+                        if constexpr (F32) O[d][t] = ORTMI_MFMA(a, PL[t], O[d][t]);
                     }
-                    sh.inv[16 * t + n] = sum != 0.f ? a / sum : 0.f;
                 }
             }
         }
+        __syncthreads();
     }
-    __syncthreads();
-    constexpr int kPieces = HD / 4;  // of a row: four channels a thread and step
-    for (int i = threadIdx.x; i < SH::kCols * kPieces; i += 256) {
-        const int c = i / kPieces, ch = 4 * (i % kPieces), r = (c0 + c) / G;
-        if (r >= s.rows) break;
-        const int64_t orow = (int64_t)(s.tok0 + r) * p.H + h * G + (c0 + c - r * G);
-        float4_t v = *reinterpret_cast<const float4_t*>(sh.rows + c * SH::kRow + ch);
-        if (nsplit > 1) {
-            if (r < s.real)
-                *reinterpret_cast<float4_t*>(p.part + (orow * p.nsplit + split) * HD + ch) = v;
-            continue;
+
+    // Each wave's columns are its own: outputs go straight to memory, neighbouring channels
+    // of a lane at once.
+    constexpr int W = HD == 128 ? 8 : 4;  // (HD 96: and two of the last third)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float sum = quarters_sum(l[t]);
+        const int c = c0 + cw + 16 * t + n, r = c / G, head = h * G + (c - r * G);
+        if (r >= s.rows) continue;
+        const int64_t row = (int64_t)(s.tok0 + r) * p.H + head;
+        const bool live = r < s.real, partial = nsplit > 1 && live;
+        if (!live && nsplit > 1 && split != 0) continue;
+        if (partial && q == 0) {
+            p.ml[(row * p.nsplit + split) * 2] = m[t];
+            p.ml[(row * p.nsplit + split) * 2 + 1] = sum;
         }
-        const float inv = r < s.real ? sh.inv[c] : 0.f;
+        const float inv = live ? output_factor<F32, PAGED>(p, head, m[t], sum) : 0.f;
+        float* part = p.part + (row * p.nsplit + split) * HD;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = inv != 0.f ? v[j] * inv * p.vs[p.v_chan ? h * HD + ch + j : 0] : 0.f;
-        if constexpr (F32) {
-            *reinterpret_cast<float4_t*>(static_cast<float*>(p.out) + orow * HD + ch) = v;
-        } else {
-            uint16_t o[4];
+        for (int i = 0; i < 4; ++i) {
+            float v[W];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                o[j] = p.dtype == ORTMI_F16 ? __builtin_bit_cast(uint16_t, (half_t)v[j])
-                                            : from_f32<uint16_t>(v[j]);
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + orow * HD + ch) =
-                *reinterpret_cast<const uint2*>(o);
+            for (int j = 0; j < W; ++j) v[j] = O[j][t][i];
+            const int ch = L::value_channel(4 * q + i, 0);
+            if (partial) {
+#pragma unroll
+                for (int j = 0; j < W; j += 4)
+                    *reinterpret_cast<float4_t*>(part + ch + j) = float4_t{v[j], v[j + 1], v[j + 2], v[j + 3]};
+            } else {
+                store_piece<W, HD, F32>(p, row, h, ch, v, inv);
+            }
+            if constexpr (HD == 96) {
+                const float z[2] = {O[4][t][i], O[5][t][i]};
+                const int ch2 = L::value_channel(4 * q + i, 4);
+                if (partial) *reinterpret_cast<float2*>(part + ch2) = make_float2(z[0], z[1]);
+                else store_piece<2, HD, F32>(p, row, h, ch2, z, inv);
+            }
         }
     }
+}
+
+// -------------------------------------------------------------------- new rows --
+// append_row in pieces: 16 lanes a row, each a sixteenth of its channels, which lie side by
+// side as their partners in the rotation do.
+template <int CODE, int HD, bool F32, bool PAGED>
+__device__ __forceinline__ void append_piece(const Params& p, int b, const Seq& s, int r, int h,
+                                             bool is_v, int lane) {
+    constexpr int N = HD / 16, RB = row_bytes(CODE, HD);
+    const int pos = s.past + r, c0 = lane * N;
+    const int64_t row = cache_row<PAGED>(p, b, h, pos);
+    const int64_t x0 = (int64_t)(s.tok0 + r) * p.kv_tok + (int64_t)h * HD;
+    const void* src = is_v ? p.v : p.k;
+    const bool rope = !is_v && p.cos, second = c0 >= HD / 2;
+    float x[N], o[N], co[N], si[N], w[N], wo[N];
+    load_piece<N, F32>(src, x0 + c0, p.dtype, x);
+    const int c1 = second ? c0 - HD / 2 : c0 + HD / 2;  // of the partners
+    if (rope) {
+        const int64_t at = min((int64_t)pos, p.max_pos - 1) * (HD / 2) + (second ? c1 : c0);
+        load_piece<N, F32>(src, x0 + c1, p.dtype, o);
+        load_piece<N, F32>(p.cos, at, p.dtype, co);
+        load_piece<N, F32>(p.sin, at, p.dtype, si);
+    }
+    double rinv = 1.0;
+    const bool norm = p.kw && !is_v;
+    if (p.kw) {  // (a value row's lanes go along)
+        double ss = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss += (double)x[i] * (double)x[i];
+#pragma unroll
+        for (int k = 8; k; k >>= 1) ss += __shfl_xor(ss, k, 64);
+        rinv = 1.0 / sqrt(ss / HD + (double)p.eps);
+        load_piece<N, F32>(p.kw, c0, p.dtype, w);
+        load_piece<N, F32>(p.kw, c1, p.dtype, wo);
+    }
+    if (row < 0) return;
+    const float* sc = (is_v ? p.vs : p.ks);
+    const bool chan = is_v ? p.v_chan : p.k_chan;
+    uint32_t u[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        double a = x[i];
+        if (norm) a = a * rinv * (double)w[i];
+        if (rope) {
+            double e = o[i];
+            if (norm) e = e * rinv * (double)wo[i];
+            const double f = a * (double)co[i], g = e * (double)si[i];
+            a = second ? f + g : f - g;
+        }
+        u[i] = encode(a, sc[chan ? h * HD + c0 + i : 0], CODE);
+    }
+    uint8_t* dst = (is_v ? p.vc : p.kc) + row * RB + (CODE == kInt4 ? c0 / 2 : c0);
+    if constexpr (CODE == kInt4) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v |= u[i] << (4 * i);
+        if constexpr (N == 8) *reinterpret_cast<uint32_t*>(dst) = v;
+        else if constexpr (N == 4) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)v;
+        else
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) dst[i] = (uint8_t)(v >> (8 * i));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2)
+            *reinterpret_cast<uint16_t*>(dst + i) = (uint16_t)(u[i] | (u[i + 1] << 8));
+    }
+}
+
+// Rows r0 .. r1 - 1 of sequence s, key and value of one kv head, by the workgroup.
+template <int CODE, int HD, bool F32, bool PAGED>
+__device__ __forceinline__ void append_rows(const Params& p, int b, const Seq& s, int r0, int r1,
+                                            int h) {
+    const int lane = threadIdx.x & 15;
+    for (int i = 2 * r0 + (int)(threadIdx.x >> 4); i < 2 * r1; i += 16) {
+        if (p.pieces) append_piece<CODE, HD, F32, PAGED>(p, b, s, i >> 1, h, i & 1, lane);
+        else append_row<PAGED>(p, b, s, i >> 1, h, i & 1, lane);
+    }
+}
+
+// The last sequence that starts at or before token `tok`, and whether it has the token.
+__device__ __forceinline__ bool sequence_of_token(const Params& p, int tok, int& b, Seq& s) {
+    int lo = 0, hi = p.B;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.cum[mid] <= tok) lo = mid;
+        else hi = mid;
+    }
+    b = lo;
+    s = sequence<true>(p, lo);
+    return tok >= s.tok0 && tok < s.tok0 + s.rows;
+}
+
+// The prompt tiles of the sequences with more than 16 columns, in order, by one wave. Ranges
+// of tokens are clamped to the call's (sequence()), and at most max_tiles are written.
+__device__ __forceinline__ void list_tiles(const Params& p) {
+    const int lane = threadIdx.x & 63, G = p.H / p.KV, w = prompt_width(p.dtype);
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int b = b0 + lane;
+        const int cols = b < p.B ? sequence<true>(p, b).rows * G : 0;
+        const int n = cols > 16 ? (cols + w - 1) / w : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += v;
+        }
+        const int first = base + incl - n;
+        for (int i = 0; i < n && first + i < p.max_tiles; ++i) p.tiles[first + i] = make_int2(b, w * i);
+        base += __shfl(incl, 63, 64);
+    }
+    if (lane == 0) *p.tile_count = min(base, p.max_tiles);
+}
+
+// New keys and values into the cache: 16 lanes per (token, kv head, key or value). Pages: the
+// first workgroup lists the tiles.
+template <int CODE, int HD, bool F32, bool PAGED>  // HD 0: any
+__global__ __launch_bounds__(256) void append_kernel(Params p) {
+    int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if constexpr (PAGED) {
+        if (blockIdx.x == 0) {
+            if (threadIdx.x < 64 && p.tiles) list_tiles(p);
+            return;
+        }
+        item -= 16;
+    }
+    const int per = 2 * p.KV;
+    const int64_t tok = item / per;
+    if (tok >= p.T) return;
+    const int hv = (int)(item % per);
+    int b;
+    Seq s;
+    if constexpr (PAGED) {
+        if (!sequence_of_token(p, (int)tok, b, s)) return;
+    } else {
+        b = (int)(tok / p.S);
+        s = sequence<false>(p, b);
+    }
+    const int r = (int)tok - s.tok0;
+    if (r >= s.real) return;
+    if constexpr (HD > 0)
+        append_piece<CODE, HD, F32, PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV, threadIdx.x & 15);
+    else
+        append_row<PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV, threadIdx.x & 15);
 }
 
 // A tile that attends nothing: padded rows.
@@ -651,42 +1019,44 @@ __device__ __forceinline__ void zero_rows(const Params& p, const Seq& s, int h, 
 }
 
 // Slabs. Workgroups: (range, tile, slab), the slab running fastest (slabs of one residue
-// modulo 8 then stay on one XCD) and later tiles, which see more keys, first. Where a
-// sequence's columns are one tile, the workgroup whose range holds the new rows writes them
-// to the cache itself.
-template <int CODE, int HD, int NT, bool F32>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void tile_kernel(Params p) {
-    __shared__ TileShared<HD, NT, F32> sh;
+// modulo 8 then stay on one XCD). Later tiles, which see more keys, come first; where all
+// workgroups run at once, two a CU, the second half runs in rising order beside them. Where a
+// sequence's columns are one tile, the workgroup whose range holds the new rows writes them to
+// the cache itself.
+template <int CODE, int HD, bool F32, bool PROMPT>
+__global__ __launch_bounds__(256, 2) void tile_kernel(Params p) {
+    using SH = std::conditional_t<PROMPT, PromptShared<CODE, HD, F32>, TokenShared<HD, F32>>;
+    __shared__ SH sh;
+    constexpr int kCols = PROMPT ? prompt_width(F32 ? ORTMI_F32 : ORTMI_F16) : 16;
     const int slabs = p.B * p.KV;
     const int split = blockIdx.x / (slabs * p.ntile), rem = blockIdx.x % (slabs * p.ntile);
-    const int tile = p.ntile - 1 - rem / slabs, slab = rem % slabs, b = slab / p.KV, h = slab % p.KV;
+    const int rank = rem / slabs, slab = rem % slabs, b = slab / p.KV, h = slab % p.KV;
+    const int upper = p.paired ? (p.ntile + 1) / 2 : p.ntile;
+    const int tile = rank < upper ? p.ntile - 1 - rank : rank - upper;
     const Seq s = sequence<false>(p, b);
-    const int G = p.H / p.KV, c0 = tile * 16 * NT;
+    const int G = p.H / p.KV, c0 = tile * kCols;
     if (c0 / G >= s.real) {
-        if (split == 0) zero_rows<HD, F32>(p, s, h, c0, 16 * NT);
+        if (split == 0) zero_rows<HD, F32>(p, s, h, c0, kCols);
         return;
     }
-    const int kend = s.keys_to((min(c0 + 16 * NT, s.rows * G) - 1) / G, p.limit);
+    const int kend = s.keys_to((min(c0 + kCols, s.rows * G) - 1) / G, p.limit);
     const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, kend);
-    if (k0 >= kend) {  // not the range that writes the rows past the sequence's end
-        return;
-    }
+    if (k0 >= kend) return;
     if (p.fused) {
-        const int r0 = max(k0 - s.past, 0), r1 = min(k1 - s.past, s.real);
-        for (int i = 2 * r0 + uniform(threadIdx.x >> 6); i < 2 * r1; i += 4)
-            append_row<false>(p, b, s, i >> 1, h, i & 1);
+        append_rows<CODE, HD, F32, false>(p, b, s, max(k0 - s.past, 0), min(k1 - s.past, s.real), h);
         __syncthreads();
     }
     const int nsplit = (kend + p.chunk - 1) / p.chunk;
-    attend_tile<CODE, HD, NT, F32, false>(p, s, b, h, c0, k0, k1, split, nsplit, sh);
-    if (nsplit > 1 && split == 0 && s.real < s.rows)  // rows of the tile that only pad
-        zero_rows<HD, F32>(p, s, h, max(c0, s.real * G), c0 + 16 * NT - max(c0, s.real * G));
+    if constexpr (PROMPT)
+        prompt_tile<CODE, HD, F32, false>(p, s, b, h, c0, k0, k1, split, nsplit, sh);
+    else
+        token_tile<CODE, HD, F32, false>(p, s, b, h, k0, k1, split, nsplit, sh);
 }
 
 // Pages, sequences of at most 16 columns: workgroups (range, sequence, kv head).
 template <int CODE, int HD, bool F32>
 __global__ __launch_bounds__(256, 2) void page_token_kernel(Params p) {
-    __shared__ TileShared<HD, 1, F32> sh;
+    __shared__ TokenShared<HD, F32> sh;
     const int slabs = p.B * p.KV, split = blockIdx.x / slabs, slab = blockIdx.x % slabs;
     const int b = slab / p.KV, h = slab % p.KV, G = p.H / p.KV;
     const Seq s = sequence<true>(p, b);
@@ -694,45 +1064,50 @@ __global__ __launch_bounds__(256, 2) void page_token_kernel(Params p) {
     const int kend = s.keys_to(s.rows - 1, p.limit);
     const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, kend);
     if (k0 >= kend) return;
-    attend_tile<CODE, HD, 1, F32, true>(p, s, b, h, 0, k0, k1, split,
-                                        (kend + p.chunk - 1) / p.chunk, sh);
+    token_tile<CODE, HD, F32, true>(p, s, b, h, k0, k1, split, (kend + p.chunk - 1) / p.chunk, sh);
 }
 
 // Pages, the other sequences: a workgroup for each (range, listed tile, kv head), those past
 // the list's end with nothing to do.
 template <int CODE, int HD, bool F32>
-__global__ __launch_bounds__(256, 1) void page_tile_kernel(Params p) {
-    constexpr int NT = page_width(F32 ? ORTMI_F32 : ORTMI_F16) / 16;
-    __shared__ TileShared<HD, NT, F32> sh;
+__global__ __launch_bounds__(256, 2) void page_tile_kernel(Params p) {
+    constexpr int kCols = prompt_width(F32 ? ORTMI_F32 : ORTMI_F16);
+    __shared__ PromptShared<CODE, HD, F32> sh;
     const int G = p.H / p.KV, per = p.max_tiles * p.KV;
     const int split = blockIdx.x / per, rem = blockIdx.x % per, h = rem % p.KV, i = rem / p.KV;
     if (i >= *p.tile_count) return;
     const int2 tl = p.tiles[i];
     const int b = tl.x, c0 = tl.y;
     const Seq s = sequence<true>(p, b);
-    const int kend = s.keys_to((min(c0 + 16 * NT, s.rows * G) - 1) / G, p.limit);
+    const int kend = s.keys_to((min(c0 + kCols, s.rows * G) - 1) / G, p.limit);
     const int k0 = split * p.tile_chunk, k1 = min(k0 + p.tile_chunk, kend);
     if (k0 >= kend) return;
-    attend_tile<CODE, HD, NT, F32, true>(p, s, b, h, c0, k0, k1, split,
-                                        (kend + p.tile_chunk - 1) / p.tile_chunk, sh);
+    prompt_tile<CODE, HD, F32, true>(p, s, b, h, c0, k0, k1, split,
+                                     (kend + p.tile_chunk - 1) / p.tile_chunk, sh);
 }
 
-// Launches for one code; in kvq_int8.hip, kvq_int4.hip and kvq_fp8.hip.
+// New rows and attention for one code; in kvq_int8.hip, kvq_int4.hip and kvq_fp8.hip.
 int tiles_int8(const Params& p, bool paged, hipStream_t st);
 int tiles_int4(const Params& p, bool paged, hipStream_t st);
 int tiles_fp8(const Params& p, bool paged, hipStream_t st);
 
 template <int CODE, int HD, bool F32>
 int launch_tiles(const Params& p, bool paged, hipStream_t st) {
+    const int G = p.H / p.KV;
+    const dim3 rows((unsigned)(((int64_t)p.T * 2 * p.KV + 15) / 16 + (paged ? 1 : 0)));
+    if (p.pieces && !p.fused) {
+        if (paged) hipLaunchKernelGGL((append_kernel<CODE, HD, F32, true>), rows, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((append_kernel<CODE, HD, F32, false>), rows, dim3(256), 0, st, p);
+        if (int rc = check_launch("kv append")) return rc;
+    }
     if (!paged) {
         const dim3 grid((unsigned)(p.B * p.KV * p.ntile * p.nsplit));
-        const int w = tile_width(p.S * (p.H / p.KV), p.dtype);
-        if (w == 16) hipLaunchKernelGGL((tile_kernel<CODE, HD, 1, F32>), grid, dim3(256), 0, st, p);
-        else if (w == 32) hipLaunchKernelGGL((tile_kernel<CODE, HD, 2, F32>), grid, dim3(256), 0, st, p);
-        else if constexpr (!F32) hipLaunchKernelGGL((tile_kernel<CODE, HD, 4, F32>), grid, dim3(256), 0, st, p);
+        if (p.S * G <= 16)
+            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, false>), grid, dim3(256), 0, st, p);
+        else
+            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, true>), grid, dim3(256), 0, st, p);
         return check_launch("kv tiles");
     }
-    const int G = p.H / p.KV;
     if (G <= 16) {
         hipLaunchKernelGGL((page_token_kernel<CODE, HD, F32>),
                            dim3((unsigned)(p.B * p.KV * p.nsplit)), dim3(256), 0, st, p);
