@@ -52,7 +52,6 @@ struct Params {
     int max_tiles;
     int* tile_count;
     int tile_chunk, tile_nsplit;  // pages: ranges of those tiles, at most nsplit of them
-    int paired;                   // slabs: two tiles a CU run at once
 };
 
 __device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {

@@ -201,7 +201,7 @@ static void plan_slabs(int64_t B, int64_t S, int64_t H, int64_t KV, int64_t n, i
     const int64_t cols = S * (H / KV);
     const int w = tile_width((int)std::min<int64_t>(cols, 1 << 20), dtype);
     ntile = (int)((cols + w - 1) / w);
-    plan_ranges(B * KV * ntile, n, w == 16 ? 768 : 512, nsplit, chunk);
+    plan_ranges(B * KV * ntile, n, w == 16 ? 768 : 256, nsplit, chunk);
 }
 
 static void plan_pages(int64_t B, int64_t KV, int64_t n, int& nsplit, int& chunk) {
@@ -236,7 +236,6 @@ static int attend(Params& p, hipStream_t st) {
                        (!PAGED || (p.blk % 16 == 0 && p.nblk <= INT32_MAX / p.blk));
     if (!tiles) p.tiles = nullptr;
     p.fused = !PAGED && tiles && p.ntile == 1;
-    p.paired = p.B * p.KV * p.ntile <= 2 * device_cu_count();
     for (const void* x : {p.k, p.v, p.cos, p.sin, p.kw}) bits |= reinterpret_cast<uintptr_t>(x);
     p.pieces = tiles && (bits & 15) == 0 && (!p.cos || (2 * p.half == p.hd && !p.interleaved));
     if (!p.fused && !p.pieces) {

@@ -22,9 +22,11 @@
 // wave decodes its own. Memory binds it: 4 sequences of 131072 int8 keys, 8 heads of 128, 190
 // us, 5.65 TB/s.
 //
-// Prompt tiles: 128 columns (fp32 64), 32 a wave, over blocks of 64 keys which the 4 waves
-// decode together into LDS, a quarter each, in the order that the products read: decoded once
-// for 128 columns. Two buffers, so that one barrier a block suffices, and two workgroups a CU.
+// Prompt tiles: 128 columns (fp32 64), 32 a wave, by two teams of 4 waves that take every other
+// block of 64 keys and are joined at the end. A team decodes its block together into LDS, a
+// quarter each, in the order that the products read: decoded once for 128 columns. Two buffers
+// a team, so that one barrier for two blocks suffices; the second team fills the waits of the
+// first, which the registers (200 of 256 at two waves a SIMD) leave no other wave for.
 #pragma once
 
 #include "kvq.h"
@@ -74,13 +76,23 @@ struct Layout {
     static constexpr int KW = RB / 16;      // words of a key row per lane
     static constexpr int VW = HD == 96 ? 2 : (RB == 128 ? 2 : 1);  // words of a value row per lane
 
-    // Channel of element j of k step ks in the lanes of quarter q.
-    __device__ static __forceinline__ int key_channel(int q, int ks, int j) {
-        const int jj = kNib ? (j >> 1) + 4 * (j & 1) : j;
-        if constexpr (HD == 128)
-            return kNib ? 32 * q + 8 * ks + jj : 64 * (ks >> 1) + 16 * q + 8 * (ks & 1) + jj;
-        else
-            return ks < 2 ? 16 * q + 8 * ks + jj : 64 + 8 * q + jj;
+    // Channel jj (of 8) of k step ks in the lanes of quarter q: HD 128, codes of a byte: 64
+    // (ks / 2) + 16 q + 8 (ks % 2) + jj; of a nibble: 32 q + 8 ks + jj; else 16 q + 8 ks + jj,
+    // and 64 + 8 q + jj in the third step of 96. A word of nibbles gives jj in the order 0, 4,
+    // 1, 5, 2, 6, 3, 7.
+    // The place of channel c in a column's [k step][quarter][8] operand.
+    __device__ static __forceinline__ int key_slot(int c) {
+        int q, ks;
+        const int jj = c & 7;
+        if constexpr (HD == 128) {
+            q = kNib ? c >> 5 : (c >> 4) & 3;
+            ks = kNib ? (c >> 3) & 3 : 2 * (c >> 6) + ((c >> 3) & 1);
+        } else {
+            q = c < 64 ? c >> 4 : (c - 64) >> 3;
+            ks = c < 64 ? (c >> 3) & 1 : 2;
+        }
+        const int j = kNib ? ((jj & 3) << 1) | (jj >> 2) : jj;
+        return (ks * 4 + q) * 8 + j;
     }
     // Byte at which the lanes of quarter q begin in a key row (and, HD 96, in its last third).
     static constexpr int kKeyStep = RB == 48 || RB == 32 ? 8 : 16;
@@ -244,18 +256,8 @@ struct Source {
     }
 };
 
-constexpr int kPass = 2;  // groups of 16 columns whose queries are staged at once
 template <int HD>
 constexpr int kRowFloats = HD + 4;  // of a row in LDS: four more than a multiple of the banks
-
-// Queries of 16 NC columns, their halves (where split), factors and positions.
-template <int HD, int NC, bool SPLIT>
-struct Queries {
-    static constexpr int kCols = 16 * NC, kStage = NC < kPass ? NC : kPass;
-    // Rows of a pass and their cos/sin.
-    __align__(16) float rows[2 * 16 * kStage * kRowFloats<HD>];
-    __align__(16) half_t q[(SPLIT ? 2 : 1) * kCols * HD];
-};
 
 // N consecutive elements of a 16-byte aligned row as fp32.
 template <int N, bool F32>
@@ -290,108 +292,95 @@ __device__ __forceinline__ float load_one(const void* base, int64_t at, int dtyp
     return dtype == ORTMI_F16 ? (float)__builtin_bit_cast(half_t, u) : to_f32(u);
 }
 
-// The query rows of columns c0 .. c0 + 16 NC - 1 into LDS, 16 lanes a column: (normalised and)
-// rotated, times the key scales, brought to [2^10, 2^11) and rounded to fp16, in the order
-// [column][k step][quarter][8] of the right operand (the second halves behind). f: what a
-// product is to be multiplied by; pos: the column's position, -1 for none.
-template <int CODE, int HD, int NC, bool F32, bool SPLIT>
+// The query rows of columns c0 .. c0 + GR NC - 1 into LDS, 16 lanes a column, each a sixteenth
+// of its channels: (normalised and) rotated, times the key scales, brought to [2^10, 2^11) and
+// rounded to fp16, in the order [column][k step][quarter][8] of the right operand (SPLIT: the
+// second halves behind). f: what a product is to be multiplied by; pos: the column's position,
+// -1 for none. The code is kept short: a workgroup runs it once, from a cold cache.
+template <int CODE, int HD, int GR, int NC, bool F32, bool SPLIT>
 __device__ __forceinline__ void stage_queries(const Params& p, const Seq& s, int h, int c0,
-                                              Queries<HD, NC, SPLIT>& sh, float* f, int* pos) {
+                                              half_t* sq, float* f, int* pos) {
     using L = Layout<CODE, HD>;
-    using SH = Queries<HD, NC, SPLIT>;
-    constexpr int N = HD / 16, R = kRowFloats<HD>, F = HD / 32;
+    constexpr int N = HD / 16;
     const int G = p.H / p.KV, tid = threadIdx.x, lane = tid & 15, group = tid >> 4;
-    const bool rope = p.cos != nullptr;
-    float x[NC][N], cs[NC][2 * F];
+    const int ch = lane * N;
+    const bool second = ch >= HD / 2;
+    const int other = second ? ch - HD / 2 : ch + HD / 2;
+    float x[NC][N], o[NC][N], co[NC][N], si[NC][N];
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
-        const int c = 16 * cc + group, r = (c0 + c) / G, g = (c0 + c) - r * G;
+        const int c = GR * cc + group, r = (c0 + c) / G, g = (c0 + c) - r * G;
         const bool live = r < s.real;
         const int tok = s.tok0 + (live ? r : 0), at = s.past + (live ? r : 0);
-        load_piece<N, F32>(p.q, (int64_t)tok * p.q_tok + (int64_t)(h * G + g) * HD + lane * N,
-                           p.dtype, x[cc]);
-        if (rope) {
-            const int64_t prow = min((int64_t)at, p.max_pos - 1) * p.half;
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                const int64_t k = prow + min(lane + 16 * i, p.half - 1);
-                cs[cc][2 * i] = load_one<F32>(p.cos, k, p.dtype);
-                cs[cc][2 * i + 1] = load_one<F32>(p.sin, k, p.dtype);
-            }
+        const int64_t x0 = (int64_t)tok * p.q_tok + (int64_t)(h * G + g) * HD;
+        load_piece<N, F32>(p.q, x0 + ch, p.dtype, x[cc]);
+        if (p.cos && p.pieces) {
+            const int64_t k = min((int64_t)at, p.max_pos - 1) * (HD / 2) + (second ? other : ch);
+            load_piece<N, F32>(p.q, x0 + other, p.dtype, o[cc]);
+            load_piece<N, F32>(p.cos, k, p.dtype, co[cc]);
+            load_piece<N, F32>(p.sin, k, p.dtype, si[cc]);
         }
         if (lane == 0) pos[c] = live ? at : -1;
     }
-    if (p.qw) {
-        float w[N];
-        load_piece<N, F32>(p.qw, lane * N, p.dtype, w);
+    float sc[N];
 #pragma unroll
-        for (int cc = 0; cc < NC; ++cc) {
+    for (int i = 0; i < N; ++i) sc[i] = p.ks[p.k_chan ? h * HD + ch + i : 0];
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc) {
+        const int c = GR * cc + group, r = (c0 + c) / G, g = (c0 + c) - r * G;
+        const bool live = r < s.real;
+        float rinv = 1.f;
+        if (p.qw) {
             float ss = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i) ss += x[cc][i] * x[cc][i];
-            const float rinv = 1.f / sqrtf(group_sum<16>(ss) / (float)HD + p.eps);
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[cc][i] = x[cc][i] * rinv * w[i];
+            rinv = 1.f / sqrtf(group_sum<16>(ss) / (float)HD + p.eps);
         }
-    }
-    // Element e of a column is channel ch[e]; the channels and scales serve every column.
-    int ch[N];
-    float sc[N];
+        if (p.pieces) {
+            if (p.qw) {
+                float w[N];
+                load_piece<N, F32>(p.qw, ch, p.dtype, w);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int e = lane * N + i;
-        ch[i] = L::key_channel((e >> 3) & 3, e >> 5, e & 7);
-        sc[i] = p.ks[p.k_chan ? h * HD + ch[i] : 0];
-    }
+                for (int i = 0; i < N; ++i) x[cc][i] = x[cc][i] * rinv * w[i];
+                if (p.cos) {
+                    load_piece<N, F32>(p.qw, other, p.dtype, w);
 #pragma unroll
-    for (int c1 = 0; c1 < NC; c1 += SH::kStage) {
-        if (c1) __syncthreads();
-#pragma unroll
-        for (int cc = 0; cc < SH::kStage; ++cc) {
-            float* row = sh.rows + (16 * cc + group) * R;
-            float* turn = sh.rows + (16 * (SH::kStage + cc) + group) * R;
-#pragma unroll
-            for (int i = 0; i < N; ++i) row[lane * N + i] = x[c1 + cc][i];
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                turn[2 * (lane + 16 * i)] = cs[c1 + cc][2 * i];
-                turn[2 * (lane + 16 * i) + 1] = cs[c1 + cc][2 * i + 1];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int cc = 0; cc < SH::kStage; ++cc) {
-            const int c = 16 * (c1 + cc) + group;
-            const float* row = sh.rows + (16 * cc + group) * R;
-            const float* turn = sh.rows + (16 * (SH::kStage + cc) + group) * R;
-            float y[N], top = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int k = ch[i];
-                float v = row[k];
-                if (rope && k < 2 * p.half) {
-                    const bool second = p.interleaved ? (k & 1) : k >= p.half;
-                    const int t = p.interleaved ? k >> 1 : (second ? k - p.half : k);
-                    const float o = row[p.interleaved ? k ^ 1 : (second ? k - p.half : k + p.half)];
-                    v = second ? v * turn[2 * t] + o * turn[2 * t + 1]
-                               : v * turn[2 * t] - o * turn[2 * t + 1];
+                    for (int i = 0; i < N; ++i) o[cc][i] = o[cc][i] * rinv * w[i];
                 }
-                y[i] = v * sc[i];
-                top = fmaxf(top, fabsf(y[i]));
             }
-            top = group_max<16>(top);
-            // A row of zeros, or with an infinity, is taken as it is.
-            const int ex = top > 0.f && top < INFINITY ? max(-100, min(ilogbf(top), 116)) : 10;
-            const bool live = pos[c] >= 0;
+            if (p.cos) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float z = live ? ldexpf(y[i], 10 - ex) : 0.f;
-                const half_t hi = (half_t)z;
-                sh.q[c * HD + lane * N + i] = hi;
-                if constexpr (SPLIT) sh.q[(SH::kCols + c) * HD + lane * N + i] = (half_t)(z - (float)hi);
+                for (int i = 0; i < N; ++i)
+                    x[cc][i] = x[cc][i] * co[cc][i] + (second ? o[cc][i] : -o[cc][i]) * si[cc][i];
             }
-            if (lane == 0) f[c] = ldexpf(p.scale, ex - 10);
+        } else {  // any rotation: element by element
+            const int at = s.past + (live ? r : 0);
+            const int64_t x0 = (int64_t)(s.tok0 + (live ? r : 0)) * p.q_tok + (int64_t)(h * G + g) * HD;
+            const int64_t prow = min((int64_t)at, p.max_pos - 1) * p.half;
+            for (int i = 0; i < N; ++i) {
+                const float v = query_elem(p, x0, prow, rinv, ch + i);
+#pragma unroll
+                for (int j = 0; j < N; ++j) x[cc][j] = j == i ? v : x[cc][j];
+            }
         }
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[cc][i] *= sc[i];
+            top = fmaxf(top, fabsf(x[cc][i]));
+        }
+        top = group_max<16>(top);
+        // A row of zeros, or with an infinity, is taken as it is.
+        const int ex = top > 0.f && top < INFINITY ? max(-100, min(ilogbf(top), 116)) : 10;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float z = live ? ldexpf(x[cc][i], 10 - ex) : 0.f;
+            const half_t hi = (half_t)z;
+            const int at = c * HD + L::key_slot(ch + i);
+            sq[at] = hi;
+            if constexpr (SPLIT) sq[GR * NC * HD + at] = (half_t)(z - (float)hi);
+        }
+        if (lane == 0) f[c] = ldexpf(p.scale, ex - 10);
     }
     __syncthreads();
 }
@@ -468,40 +457,48 @@ __device__ __forceinline__ float output_factor(const Params& p, int head, float 
     return l != 0.f ? a / l : 0.f;
 }
 
-// N (4 or 8) neighbouring channels of an output row; a factor of 0 gives zeros whatever they are.
-template <int N, int HD, bool F32>
-__device__ __forceinline__ void store_piece(const Params& p, int64_t row, int h, int ch,
-                                            const float (&v)[N], float inv) {
+// N (2, 4 or 8) neighbouring channels of an output row, times their value scales vs; a factor
+// of 0 gives zeros whatever they are.
+template <int N, bool F32>
+__device__ __forceinline__ void store_piece(const Params& p, int64_t at, const float (&v)[N],
+                                            const float (&vs)[N], float inv) {
     float y[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-        y[j] = inv != 0.f ? v[j] * inv * p.vs[p.v_chan ? h * HD + ch + j : 0] : 0.f;
+    for (int j = 0; j < N; ++j) y[j] = inv != 0.f ? v[j] * inv * vs[j] : 0.f;
     if constexpr (F32) {
-        float* o = static_cast<float*>(p.out) + row * HD + ch;
+        float* o = static_cast<float*>(p.out) + at;
 #pragma unroll
         for (int j = 0; j < N; j += 2) *reinterpret_cast<float2*>(o + j) = make_float2(y[j], y[j + 1]);
     } else {
         uint32_t w[N / 2];
+        if (p.dtype == ORTMI_F16) {
 #pragma unroll
-        for (int j = 0; j < N / 2; ++j) {
-            const uint16_t a = p.dtype == ORTMI_F16 ? __builtin_bit_cast(uint16_t, (half_t)y[2 * j])
-                                                    : from_f32<uint16_t>(y[2 * j]);
-            const uint16_t b = p.dtype == ORTMI_F16 ? __builtin_bit_cast(uint16_t, (half_t)y[2 * j + 1])
-                                                    : from_f32<uint16_t>(y[2 * j + 1]);
-            w[j] = a | ((uint32_t)b << 16);
+            for (int j = 0; j < N / 2; ++j) {
+                const half2_t z = {(half_t)y[2 * j], (half_t)y[2 * j + 1]};
+                w[j] = __builtin_bit_cast(uint32_t, z);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j)
+                w[j] = from_f32<uint16_t>(y[2 * j]) | ((uint32_t)from_f32<uint16_t>(y[2 * j + 1]) << 16);
         }
-        uint16_t* o = static_cast<uint16_t*>(p.out) + row * HD + ch;
+        uint16_t* o = static_cast<uint16_t*>(p.out) + at;
         if constexpr (N == 8) *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
         else if constexpr (N == 4) *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
         else *reinterpret_cast<uint32_t*>(o) = w[0];
     }
+}
+template <int N>
+__device__ __forceinline__ void value_scales(const Params& p, int at, float (&vs)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) vs[j] = p.vs[p.v_chan ? at + j : 0];
 }
 
 // ----------------------------------------------------------------- token tiles --
 template <int HD, bool F32>
 struct TokenShared {
     union {
-        Queries<HD, 1, true> queries;
+        __align__(16) half_t queries[2 * 16 * HD];
         __align__(16) float4_t out[2][HD / 16][64];    // two waves' outputs
         __align__(16) float rows[16 * kRowFloats<HD>];  // the tile's output
     };
@@ -526,8 +523,8 @@ __device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b,
     int2 sl = src.slots(kb), sl_n = src.slots(kb + 128);
     Block<CODE, HD> cur, nxt;
     if (kb < k1) src.load(kb, sl, cur);
-    stage_queries<CODE, HD, 1, F32, true>(p, s, h, 0, sh.queries, sh.f, sh.pos);
-    const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries.q);
+    stage_queries<CODE, HD, 16, 1, F32, true>(p, s, h, 0, sh.queries, sh.f, sh.pos);
+    const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries);
     half8_t Q[KS], QL[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -648,7 +645,9 @@ __device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b,
             *reinterpret_cast<float4_t*>(p.part + (orow * p.nsplit + split) * HD + ch) = v;
         } else if (nsplit <= 1 || split == 0) {
             const float y[4] = {v[0], v[1], v[2], v[3]};
-            store_piece<4, HD, F32>(p, orow, h, ch, y, r < s.real ? sh.inv[c] : 0.f);
+            float vs[4];
+            value_scales(p, h * HD + ch, vs);
+            store_piece<4, F32>(p, orow * HD + ch, y, vs, r < s.real ? sh.inv[c] : 0.f);
         }
     }
 }
@@ -657,13 +656,15 @@ __device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b,
 template <int CODE, int HD, bool F32>
 struct PromptShared {
     static constexpr int kNT = F32 ? 1 : 2, kCols = 64 * kNT;
-    union {
-        Queries<HD, 4 * kNT, F32> queries;
-        struct {  // two blocks of 64 keys: [key tile][k step], [half][channel tile], by lane
-            half8_t k[2][4][HD / 32][64], v[2][2][HD / 16][64];
-        };
+    struct Blocks {  // two blocks of 64 keys: [key tile][k step], [half][channel tile], by lane
+        half8_t k[2][4][HD / 32][64], v[2][2][HD / 16][64];
     };
-    float f[kCols];
+    union {
+        __align__(16) half_t queries[(F32 ? 2 : 1) * kCols * HD];
+        Blocks team[2];
+        __align__(16) float4_t out[4][HD / 16][kNT][64];  // the second team's outputs
+    };
+    float f[kCols], m[kCols], l[kCols];
     int pos[kCols];
 };
 
@@ -676,9 +677,10 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
     using SH = PromptShared<CODE, HD, F32>;
     constexpr int KS = L::KS, MT = L::MT, NT = SH::kNT, UH = (MT / 2 + 1) / 2;
     const int lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
-    const int wave = uniform(threadIdx.x >> 6);
+    const int team = uniform(threadIdx.x >> 8), wave = uniform(threadIdx.x >> 6) & 3;
     const int G = p.H / p.KV;
     const Source<CODE, HD, PAGED> src(p, b, h, k0, k1);
+    auto& blocks = sh.team[team];
 
     // Of a block at kb a wave decodes key tile `wave`, and of the values of its half of the
     // keys (wave / 2) half of the channel tiles.
@@ -689,27 +691,29 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
         for (int t = 0; t < 4; ++t) sl[t] = src.slot(kb + 16 * t);
     };
     auto load = [&](int kb, const int (&sl)[4]) {
-        const int k = wave & 1 ? (wave & 2 ? sl[3] : sl[1]) : (wave & 2 ? sl[2] : sl[0]);
-        src.keys(kb + 16 * wave, k, rk);
-        src.values(kb + 32 * (wave >> 1), wave & 2 ? sl[2] : sl[0], wave & 2 ? sl[3] : sl[1], rv);
+        const int s0 = sl[0], s1 = sl[1], s2 = sl[2], s3 = sl[3];
+        const int a = wave & 2 ? s2 : s0, c = wave & 2 ? s3 : s1;
+        src.keys(kb + 16 * wave, wave & 1 ? c : a, rk);
+        src.values(kb + 32 * (wave >> 1), a, c, rv);
     };
     auto decode = [&](int buf) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) sh.k[buf][wave][ks][lane] = L::key_step(rk, ks);
+        for (int ks = 0; ks < KS; ++ks) blocks.k[buf][wave][ks][lane] = L::key_step(rk, ks);
 #pragma unroll
         for (int u = 0; u < MT / 2; ++u)
             if ((u < UH) == !(wave & 1)) {
                 half8_t a, c;
                 L::value_steps(rv, u, a, c);
-                sh.v[buf][wave >> 1][2 * u][lane] = a;
-                sh.v[buf][wave >> 1][2 * u + 1][lane] = c;
+                blocks.v[buf][wave >> 1][2 * u][lane] = a;
+                blocks.v[buf][wave >> 1][2 * u + 1][lane] = c;
             }
     };
 
-    slots(k0, slot);
-    load(k0, slot);
-    stage_queries<CODE, HD, 4 * NT, F32, F32>(p, s, h, c0, sh.queries, sh.f, sh.pos);
-    const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries.q);
+    int kb = k0 + 64 * team;
+    slots(kb, slot);
+    if (kb < k1) load(kb, slot);
+    stage_queries<CODE, HD, 32, 2 * NT, F32, F32>(p, s, h, c0, sh.queries, sh.f, sh.pos);
+    const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries);
     half8_t Q[NT][KS], QL[F32 ? NT : 1][KS];
     float f[NT];
     int pos[NT];
@@ -739,21 +743,21 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
         for (int d = 0; d < MT; ++d) O[d][t] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     __syncthreads();  // the queries are read: the blocks take their place
-    decode(0);
-    slots(k0 + 64, slot_n);
-    if (k0 + 64 < k1) load(k0 + 64, slot_n);
+    if (kb < k1) decode(0);
+    slots(kb + 128, slot_n);
+    if (kb + 128 < k1) load(kb + 128, slot_n);
     __syncthreads();
     int buf = 0;
-    for (int kb = k0; kb < k1; kb += 64, buf ^= 1) {
+    for (int first_kb = k0; first_kb < k1; first_kb += 128, kb += 128, buf ^= 1) {
         const int sl[4] = {slot[0], slot[1], slot[2], slot[3]};
-        if (kb + 64 < k1) {
+        if (kb + 128 < k1) {
             decode(buf ^ 1);
 #pragma unroll
             for (int t = 0; t < 4; ++t) slot[t] = slot_n[t];
-            slots(kb + 128, slot_n);
-            if (kb + 128 < k1) load(kb + 128, slot_n);
+            slots(kb + 256, slot_n);
+            if (kb + 256 < k1) load(kb + 256, slot_n);
         }
-        if (kb <= last) {
+        if (kb <= last && kb < k1) {
             float x[NT][4][4];
 #pragma unroll
             for (int t4 = 0; t4 < 4; ++t4) {
@@ -762,7 +766,7 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
                 for (int t = 0; t < NT; ++t) S[t] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const half8_t a = sh.k[buf][t4][ks][lane];
+                    const half8_t a = blocks.k[buf][t4][ks][lane];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
                         S[t] = ORTMI_MFMA(a, Q[t][ks], S[t]);
@@ -809,7 +813,7 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
                     probabilities<F32>(x[t][2 * j], x[t][2 * j + 1], m[t], l[t], P[t], PL[t]);
 #pragma unroll
                 for (int d = 0; d < MT; ++d) {
-                    const half8_t a = sh.v[buf][j][d][lane];
+                    const half8_t a = blocks.v[buf][j][d][lane];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
                         O[d][t] = ORTMI_MFMA(a, P[t], O[d][t]);
@@ -821,41 +825,71 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
         __syncthreads();
     }
 
-    // Each wave's columns are its own: outputs go straight to memory, neighbouring channels
-    // of a lane at once.
-    constexpr int W = HD == 128 ? 8 : 4;  // (HD 96: and two of the last third)
+    // The second team's outputs to the first, which writes them: a lane's neighbouring channels
+    // at once.
+    if (team) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float sum = quarters_sum(l[t]);
+            if (q == 0) {
+                sh.m[cw + 16 * t + n] = m[t];
+                sh.l[cw + 16 * t + n] = sum;
+            }
+#pragma unroll
+            for (int d = 0; d < MT; ++d) sh.out[wave][d][t][lane] = O[d][t];
+        }
+    }
+    __syncthreads();
+    if (team) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const float sum = quarters_sum(l[t]);
-        const int c = c0 + cw + 16 * t + n, r = c / G, head = h * G + (c - r * G);
-        if (r >= s.rows) continue;
-        const int64_t row = (int64_t)(s.tok0 + r) * p.H + head;
-        const bool live = r < s.real, partial = nsplit > 1 && live;
-        if (!live && nsplit > 1 && split != 0) continue;
-        if (partial && q == 0) {
-            p.ml[(row * p.nsplit + split) * 2] = m[t];
-            p.ml[(row * p.nsplit + split) * 2 + 1] = sum;
-        }
-        const float inv = live ? output_factor<F32, PAGED>(p, head, m[t], sum) : 0.f;
-        float* part = p.part + (row * p.nsplit + split) * HD;
+        const float m1 = sh.m[cw + 16 * t + n], mm = fmaxf(m[t], m1);
+        const float a0 = __builtin_amdgcn_exp2f(m[t] - mm), a1 = __builtin_amdgcn_exp2f(m1 - mm);
+        m[t] = mm;
+        l[t] = quarters_sum(l[t]) * a0 + sh.l[cw + 16 * t + n] * a1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int d = 0; d < MT; ++d) O[d][t] = O[d][t] * a0 + sh.out[wave][d][t][lane] * a1;
+    }
+    constexpr int W = HD == 128 ? 8 : 4;  // (HD 96: and two of the last third)
+    int64_t row[NT];
+    float inv[NT];
+    bool live[NT], partial[NT], any[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int c = c0 + cw + 16 * t + n, r = c / G, head = h * G + (c - r * G);
+        row[t] = (int64_t)(s.tok0 + r) * p.H + head;
+        live[t] = r < s.real;
+        partial[t] = nsplit > 1 && live[t];
+        any[t] = r < s.rows && (live[t] || nsplit <= 1 || split == 0);
+        if (partial[t] && q == 0) {
+            p.ml[(row[t] * p.nsplit + split) * 2] = m[t];
+            p.ml[(row[t] * p.nsplit + split) * 2 + 1] = l[t];
+        }
+        inv[t] = live[t] ? output_factor<F32, PAGED>(p, head, m[t], l[t]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int ch = L::value_channel(4 * q + i, 0), ch2 = L::value_channel(4 * q + i, MT - 2);
+        float vs[W], vs2[2];
+        value_scales(p, h * HD + ch, vs);
+        if constexpr (HD == 96) value_scales(p, h * HD + ch2, vs2);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (!any[t]) continue;
             float v[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) v[j] = O[j][t][i];
-            const int ch = L::value_channel(4 * q + i, 0);
-            if (partial) {
+            const float z[2] = {O[MT - 2][t][i], O[MT - 1][t][i]};
+            if (partial[t]) {
+                float* part = p.part + (row[t] * p.nsplit + split) * HD;
 #pragma unroll
                 for (int j = 0; j < W; j += 4)
                     *reinterpret_cast<float4_t*>(part + ch + j) = float4_t{v[j], v[j + 1], v[j + 2], v[j + 3]};
+                if constexpr (HD == 96)
+                    *reinterpret_cast<float2*>(part + ch2) = make_float2(z[0], z[1]);
             } else {
-                store_piece<W, HD, F32>(p, row, h, ch, v, inv);
-            }
-            if constexpr (HD == 96) {
-                const float z[2] = {O[4][t][i], O[5][t][i]};
-                const int ch2 = L::value_channel(4 * q + i, 4);
-                if (partial) *reinterpret_cast<float2*>(part + ch2) = make_float2(z[0], z[1]);
-                else store_piece<2, HD, F32>(p, row, h, ch2, z, inv);
+                store_piece<W, F32>(p, row[t] * HD + ch, v, vs, inv[t]);
+                if constexpr (HD == 96) store_piece<2, F32>(p, row[t] * HD + ch2, z, vs2, inv[t]);
             }
         }
     }
@@ -932,7 +966,7 @@ template <int CODE, int HD, bool F32, bool PAGED>
 __device__ __forceinline__ void append_rows(const Params& p, int b, const Seq& s, int r0, int r1,
                                             int h) {
     const int lane = threadIdx.x & 15;
-    for (int i = 2 * r0 + (int)(threadIdx.x >> 4); i < 2 * r1; i += 16) {
+    for (int i = 2 * r0 + (int)(threadIdx.x >> 4); i < 2 * r1; i += (int)(blockDim.x >> 4)) {
         if (p.pieces) append_piece<CODE, HD, F32, PAGED>(p, b, s, i >> 1, h, i & 1, lane);
         else append_row<PAGED>(p, b, s, i >> 1, h, i & 1, lane);
     }
@@ -1009,7 +1043,7 @@ __global__ __launch_bounds__(256) void append_kernel(Params p) {
 template <int HD, bool F32>
 __device__ __forceinline__ void zero_rows(const Params& p, const Seq& s, int h, int c0, int cols) {
     const int G = p.H / p.KV;
-    for (int i = threadIdx.x; i < cols * HD; i += 256) {
+    for (int i = threadIdx.x; i < cols * HD; i += blockDim.x) {
         const int c = c0 + i / HD, r = c / G;
         if (r >= s.rows) break;
         const int64_t o = ((int64_t)(s.tok0 + r) * p.H + h * G + (c - r * G)) * HD + i % HD;
@@ -1019,20 +1053,17 @@ __device__ __forceinline__ void zero_rows(const Params& p, const Seq& s, int h, 
 }
 
 // Slabs. Workgroups: (range, tile, slab), the slab running fastest (slabs of one residue
-// modulo 8 then stay on one XCD). Later tiles, which see more keys, come first; where all
-// workgroups run at once, two a CU, the second half runs in rising order beside them. Where a
+// modulo 8 then stay on one XCD). Later tiles, which see more keys, come first. Where a
 // sequence's columns are one tile, the workgroup whose range holds the new rows writes them to
 // the cache itself.
 template <int CODE, int HD, bool F32, bool PROMPT>
-__global__ __launch_bounds__(256, 2) void tile_kernel(Params p) {
+__global__ __launch_bounds__(PROMPT ? 512 : 256, 2) void tile_kernel(Params p) {
     using SH = std::conditional_t<PROMPT, PromptShared<CODE, HD, F32>, TokenShared<HD, F32>>;
     __shared__ SH sh;
     constexpr int kCols = PROMPT ? prompt_width(F32 ? ORTMI_F32 : ORTMI_F16) : 16;
     const int slabs = p.B * p.KV;
     const int split = blockIdx.x / (slabs * p.ntile), rem = blockIdx.x % (slabs * p.ntile);
-    const int rank = rem / slabs, slab = rem % slabs, b = slab / p.KV, h = slab % p.KV;
-    const int upper = p.paired ? (p.ntile + 1) / 2 : p.ntile;
-    const int tile = rank < upper ? p.ntile - 1 - rank : rank - upper;
+    const int tile = p.ntile - 1 - rem / slabs, slab = rem % slabs, b = slab / p.KV, h = slab % p.KV;
     const Seq s = sequence<false>(p, b);
     const int G = p.H / p.KV, c0 = tile * kCols;
     if (c0 / G >= s.real) {
@@ -1070,7 +1101,7 @@ __global__ __launch_bounds__(256, 2) void page_token_kernel(Params p) {
 // Pages, the other sequences: a workgroup for each (range, listed tile, kv head), those past
 // the list's end with nothing to do.
 template <int CODE, int HD, bool F32>
-__global__ __launch_bounds__(256, 2) void page_tile_kernel(Params p) {
+__global__ __launch_bounds__(512, 2) void page_tile_kernel(Params p) {
     constexpr int kCols = prompt_width(F32 ? ORTMI_F32 : ORTMI_F16);
     __shared__ PromptShared<CODE, HD, F32> sh;
     const int G = p.H / p.KV, per = p.max_tiles * p.KV;
@@ -1105,7 +1136,7 @@ int launch_tiles(const Params& p, bool paged, hipStream_t st) {
         if (p.S * G <= 16)
             hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, false>), grid, dim3(256), 0, st, p);
         else
-            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, true>), grid, dim3(256), 0, st, p);
+            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, true>), grid, dim3(512), 0, st, p);
         return check_launch("kv tiles");
     }
     if (G <= 16) {
@@ -1115,7 +1146,7 @@ int launch_tiles(const Params& p, bool paged, hipStream_t st) {
     }
     if ((int64_t)p.T * G <= 16) return ORTMI_OK;  // no sequence has more than 16 columns
     hipLaunchKernelGGL((page_tile_kernel<CODE, HD, F32>),
-                       dim3((unsigned)(p.max_tiles * p.KV * p.tile_nsplit)), dim3(256), 0, st, p);
+                       dim3((unsigned)(p.max_tiles * p.KV * p.tile_nsplit)), dim3(512), 0, st, p);
     return check_launch("kv page tiles");
 }
 
