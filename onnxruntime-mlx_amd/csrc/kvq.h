@@ -40,18 +40,22 @@ struct Params {
     const void* sink;           // [H], or null
     int dtype, code;
     void* out;                  // [T, H * hd]
-    // Ranges of `chunk` keys (a multiple of 128): nsplit of them at most. Rows over more than
-    // one leave outputs part [T * H][nsplit][hd], maxima and sums ml [T * H][nsplit][2].
-    int nsplit, chunk;
-    float *part, *ml;
-    int ntile;                  // slabs: tiles of a sequence's columns
+    // Keys are taken in ranges of whole 128s. A unit is one range of one tile of columns and kv
+    // head; units of tiles with more than one range leave outputs part [unit][columns][hd],
+    // maxima and sums ml [unit][columns][2], unscaled.
+    float *part, *ml;           // of token tiles, and of slabs' prompt tiles
+    int tcols;                  // columns of a token tile's unit there
+    int titems, tmin;           // token tiles: units over KV to come near, least keys of a range
+    int ntile, nsplit, chunk;   // slabs: tiles of a sequence, ranges of `chunk` keys at most
+    int planned;                // slabs, token tiles: ranges from the sequences' lengths
+    float *ppart, *pml;         // pages: of prompt tiles
+    int pitems, pmin;           // prompt tiles: units over KV to come near, least keys of a range
+    int4* plan;                 // pages: plan_units()
+    int tgrid, pgrid;           // units over KV at most
     int fused;                  // slabs: the tiles write the new rows themselves
     int pieces;                 // new rows come in 16-byte pieces, rotated over the whole head
-    int blk_shift;              // pages: log2(blk), or -1
-    int2* tiles;                // pages: (sequence, first column) of prompt tiles
-    int max_tiles;
-    int* tile_count;
-    int tile_chunk, tile_nsplit;  // pages: ranges of those tiles, at most nsplit of them
+    uint32_t blk_mul;           // pages of whole key tiles: division by blk (Source)
+    int blk_shift;
 };
 
 __device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {

@@ -8,58 +8,81 @@
 namespace ortmi {
 namespace kvq {
 
-// Joins the ranges of the rows whose tile had more than one: a wave per (token, head).
-template <bool PAGED>
+// Joins the ranges of tiles that have more than one: a workgroup for each unit, which takes its
+// share of the tile's columns (of prompt tiles, eight for each unit). A column's ranges are read
+// by 2, 4 or 8 half-waves, float4 a lane, and joined through LDS: many ranges of few columns and
+// few of many keep all lanes busy.
+constexpr int kShares = 8;
+template <bool F32, bool PAGED>
 __global__ __launch_bounds__(256) void merge_kernel(Params p) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)p.T * p.H) return;
-    const int lane = threadIdx.x & 63, tok = (int)(row / p.H), head = (int)(row % p.H);
-    const int G = p.H / p.KV, h = head / G;
-    int b;
+    __shared__ float4_t acc_s[8][32];
+    constexpr int kW = prompt_width(F32 ? ORTMI_F32 : ORTMI_F16);
+    const int G = p.H / p.KV;
+    Unit un;
     Seq s;
+    int cols = p.tcols, shares = 1, share = 0;  // (cols: of a unit in part and ml)
+    bool any;
     if constexpr (PAGED) {
-        if (!sequence_of_token(p, tok, b, s)) return;
+        const int i = (int)blockIdx.x / p.KV, h = (int)blockIdx.x % p.KV;
+        if (i < p.tgrid) {
+            any = page_unit<F32, false>(p, i, h, un, s);
+        } else {
+            share = (i - p.tgrid) % kShares;
+            shares = kShares;
+            any = page_unit<F32, true>(p, (i - p.tgrid) / kShares, h, un, s);
+        }
+    } else if (p.S * G <= 16) {
+        any = slab_unit<F32, false>(p, blockIdx.x, un, s);
     } else {
-        b = tok / p.S;
-        s = sequence<false>(p, b);
+        share = blockIdx.x % kShares;
+        shares = kShares;
+        any = slab_unit<F32, true>(p, blockIdx.x / kShares, un, s);
     }
-    const int r = tok - s.tok0, cols = s.rows * G;
-    if (r >= s.real) return;
-    const int w = tile_width(cols, p.dtype);
-    const int c0 = (r * G + head - h * G) / w * w;
-    const int kend = s.keys_to((min(c0 + w, cols) - 1) / G, p.limit);
-    const int chunk = PAGED && cols > 16 ? p.tile_chunk : p.chunk;
-    const int n = (kend + chunk - 1) / chunk;
-    if (n <= 1) return;
-    const float* ml = p.ml + row * p.nsplit * 2;
-    float top = kNone;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, ml[2 * i]);
-    top = wave_max(top);
-    float a = 1.f, sum = 0.f;
-    for (int i = lane; i < n; i += 64) sum += ml[2 * i + 1] * __builtin_amdgcn_exp2f(ml[2 * i] - top);
-    sum = wave_sum(sum);
-    if (PAGED && p.sink) {
-        const float sk = load_elem(p.sink, head, p.dtype) * 1.44269504088896341f;
-        const float mm = fmaxf(top, sk);
-        a = __builtin_amdgcn_exp2f(top - mm);
-        sum = sum * a + __builtin_amdgcn_exp2f(sk - mm + kPBase);
-    }
-    const float inv = sum != 0.f ? a / sum : 0.f;
-    float acc[2] = {0.f, 0.f};
-    const float* o = p.part + row * p.nsplit * p.hd;
+    if (!any || un.n <= 1) return;
+    if (shares > 1) cols = kW;
+    const int n = un.n, live = min(cols, s.real * G - un.c0);
+    // Of the columns, part `at` of n * shares.
+    const int at = un.split * shares + share;
+    const int end = (int)((int64_t)live * (at + 1) / (n * shares));
+    const int per = n > 16 ? 8 : n > 4 ? 4 : 2;  // half-waves a column
+    const int hw = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = 4 * lane;
+    for (int c0 = (int)((int64_t)live * at / (n * shares)); c0 < end; c0 += 8 / per) {
+        const int c = min(c0 + hw / per, end - 1), sub = hw % per;
+        float top = kNone;
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, un.ml[un.row(i, cols, c) * 2]);
+        top = group_max<32>(top);
+        float sum = 0.f;
+        float4_t acc{0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            float w = 0.f;
+            if (i0 + lane < n) {
+                const float2 ml = reinterpret_cast<const float2*>(un.ml)[un.row(i0 + lane, cols, c)];
+                w = __builtin_amdgcn_exp2f(ml.x - top);
+                sum += w * ml.y;
+            }
+            const int m = min(32, n - i0);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float e = __builtin_amdgcn_exp2f(ml[2 * i] - top);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (64 * j + lane < p.hd) acc[j] += e * o[(int64_t)i * p.hd + 64 * j + lane];
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int ch = 64 * j + lane;
-        if (ch >= p.hd) break;
-        const float y = inv != 0.f ? acc[j] * inv * p.vs[p.v_chan ? h * p.hd + ch : 0] : 0.f;
-        store_elem(p.out, row * p.hd + ch, y, p.dtype);
+            for (int j = 0; j < m; j += per) {
+                const int i = j + sub;  // (at most 31)
+                const float e = __shfl(w, i, 32);
+                if (ch < p.hd && i < m)
+                    acc += e * *reinterpret_cast<const float4_t*>(
+                                   un.part + un.row(i0 + i, cols, c) * p.hd + ch);
+            }
+        }
+        sum = group_sum<32>(sum);
+        __syncthreads();
+        acc_s[hw][lane] = acc;
+        __syncthreads();
+        const int col = un.c0 + c, r = col / G, head = un.h * G + (col - r * G);
+        if (sub == 0 && ch < p.hd && c0 + hw / per < end) {
+            for (int i = 1; i < per; ++i) acc += acc_s[hw + i][lane];
+            float vs[4];
+            load_scales<4>(p.vs, p.v_chan, un.h * p.hd + ch, vs);
+            const float y[4] = {acc[0], acc[1], acc[2], acc[3]};
+            store_piece<4, F32>(p, ((int64_t)(s.tok0 + r) * p.H + head) * p.hd + ch, y, vs,
+                                output_factor<F32, PAGED>(p, head, top, sum));
+        }
     }
 }
 
@@ -196,33 +219,64 @@ static void plan_ranges(int64_t wgs, int64_t n, int64_t target, int& nsplit, int
 static bool tile_head(int64_t hd) { return hd == 64 || hd == 96 || hd == 128; }
 static size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
-static void plan_slabs(int64_t B, int64_t S, int64_t H, int64_t KV, int64_t n, int dtype,
-                       int& ntile, int& nsplit, int& chunk) {
-    const int64_t cols = S * (H / KV);
-    const int w = tile_width((int)std::min<int64_t>(cols, 1 << 20), dtype);
-    ntile = (int)((cols + w - 1) / w);
-    plan_ranges(B * KV * ntile, n, w == 16 ? 768 : 256, nsplit, chunk);
+// Units that token and prompt tiles are cut into, where there are keys enough: three workgroups
+// of token tiles fit on a CU, and two rounds of them even out what differs (32 int8 sequences of
+// 256 to 8192 keys: 512 units 78 us, 768 72, 1536 64; 16 int4 ones of up to 32768: 124, 120,
+// 102), but a range of fewer than 512 keys is mostly start and end (eight of 4096: 512 keys 21
+// us, 171 27), and a lone sequence that short needs no join. One workgroup of prompt tiles fills
+// a CU: as many units as CUs, since each has about 12 us around its loop.
+constexpr int64_t kTokenUnits = 1536, kPromptUnits = 256;
+constexpr int kTokenLeast = 512, kPromptLeast = 256;
+
+// The ranges' part of the workspace, from byte `ws` of it; returns what lies behind it.
+static size_t place_parts(float*& part, float*& ml, char* ws, size_t at, int64_t rows, int64_t hd) {
+    part = reinterpret_cast<float*>(ws + at);
+    at += align_up((size_t)rows * hd * 4);
+    ml = reinterpret_cast<float*>(ws + at);
+    return at + align_up((size_t)rows * 8);
 }
 
-static void plan_pages(int64_t B, int64_t KV, int64_t n, int& nsplit, int& chunk) {
-    plan_ranges(B * KV, n, 4096, nsplit, chunk);
-}
-
-static int max_page_tiles(int64_t T, int64_t B, int64_t G, int w) { return (int)((T * G + w - 1) / w + B); }
-
-static size_t ranges_bytes(int64_t rows, int nsplit, int64_t hd) {
-    return nsplit > 1 ? align_up((size_t)rows * nsplit * hd * 4) + align_up((size_t)rows * nsplit * 8) : 0;
-}
-
-// The ranges' part of the workspace; returns what lies behind it.
-static char* place_ranges(Params& p, char* ws) {
-    if (p.nsplit > 1) {
-        const size_t rows = (size_t)p.T * p.H;
-        p.part = reinterpret_cast<float*>(ws);
-        p.ml = reinterpret_cast<float*>(ws + align_up(rows * p.nsplit * p.hd * 4));
-        ws += ranges_bytes((int64_t)rows, p.nsplit, p.hd);
+// Slabs: the plan of a call, and its workspace from ws on; returns the bytes.
+static size_t plan_slabs(Params& p, int64_t n, char* ws) {
+    const int64_t cols = (int64_t)p.S * (p.H / p.KV), slabs = (int64_t)p.B * p.KV;
+    const int w = tile_width((int)std::min<int64_t>(cols, 1 << 20), p.dtype);
+    p.ntile = (int)((cols + w - 1) / w);
+    p.planned = w == 16 && p.B <= 64;
+    p.tcols = (int)cols;
+    p.tmin = kTokenLeast;
+    plan_ranges(slabs * p.ntile, n, w == 16 ? kTokenUnits : kPromptUnits, p.nsplit, p.chunk);
+    if (!tile_head(p.hd)) p.planned = 0, p.nsplit = 1;
+    int64_t units = slabs * p.ntile * p.nsplit;
+    if (p.planned) {
+        const int64_t most = (n + p.tmin - 1) / p.tmin;  // ranges of a sequence
+        p.titems = (int)std::max<int64_t>(1, kTokenUnits / p.KV);
+        p.tgrid = (int)std::min<int64_t>(p.titems + p.B, p.B * std::max<int64_t>(1, most));
+        p.nsplit = most > 1 ? 2 : 1;  // (more than one, or one)
+        units = std::min<int64_t>(p.tgrid, 2 * p.titems) * p.KV;
     }
-    return ws;
+    if (p.nsplit == 1) return 0;
+    return place_parts(p.part, p.ml, ws, 0, units * (w == 16 ? cols : w), p.hd);
+}
+
+// Pages: the same.
+static size_t plan_pages(Params& p, char* ws) {
+    const int64_t G = p.H / p.KV, cols = p.T * G, w = prompt_width(p.dtype);
+    const int64_t seqs = std::min<int64_t>(p.B, p.T);
+    p.titems = (int)std::max<int64_t>(1, kTokenUnits / p.KV);
+    p.pitems = (int)std::max<int64_t>(1, kPromptUnits / p.KV);
+    p.tmin = kTokenLeast;
+    p.pmin = kPromptLeast;
+    p.tcols = (int)std::min<int64_t>(16, cols);
+    p.tgrid = G > 16 ? 0 : (int)(p.titems + seqs);
+    // Sequences with prompt tiles have 17 columns or more.
+    const int64_t tiles = cols / w + std::min<int64_t>(seqs, cols / 17);
+    p.pgrid = tiles ? (int)(p.pitems + tiles) : 0;
+    size_t at = align_up((size_t)(p.B + 1) * sizeof(int4));
+    p.plan = reinterpret_cast<int4*>(ws);
+    p.nsplit = p.limit > std::min(p.tmin, kPromptLeast) ? 2 : 1;
+    if (p.nsplit == 1) return at;
+    at = place_parts(p.part, p.ml, ws, at, std::min(p.tgrid, 2 * p.titems) * (int64_t)p.KV * p.tcols, p.hd);
+    return place_parts(p.ppart, p.pml, ws, at, std::min(p.pgrid, 2 * p.pitems) * p.KV * w, p.hd);
 }
 
 // On the matrix cores where head size and alignment allow 16-byte loads and pages are whole
@@ -234,7 +288,7 @@ static int attend(Params& p, hipStream_t st) {
         bits |= reinterpret_cast<uintptr_t>(x);
     const bool tiles = tile_head(p.hd) && (bits & 15) == 0 &&
                        (!PAGED || (p.blk % 16 == 0 && p.nblk <= INT32_MAX / p.blk));
-    if (!tiles) p.tiles = nullptr;
+    if (!tiles) p.plan = nullptr;
     p.fused = !PAGED && tiles && p.ntile == 1;
     for (const void* x : {p.k, p.v, p.cos, p.sin, p.kw}) bits |= reinterpret_cast<uintptr_t>(x);
     p.pieces = tiles && (bits & 15) == 0 && (!p.cos || (2 * p.half == p.hd && !p.interleaved));
@@ -255,8 +309,12 @@ static int attend(Params& p, hipStream_t st) {
     else if (p.code == kInt4) rc = tiles_int4(p, PAGED, st);
     else rc = tiles_fp8(p, PAGED, st);
     if (rc || p.nsplit == 1) return rc;
-    hipLaunchKernelGGL((merge_kernel<PAGED>), dim3((unsigned)(((int64_t)p.T * p.H + 3) / 4)),
-                       dim3(256), 0, st, p);
+    const int64_t shares = p.S * (p.H / p.KV) > 16 ? kShares : 1;
+    const dim3 units((unsigned)(PAGED ? (p.tgrid + (int64_t)kShares * p.pgrid) * p.KV : shares * slab_units(p)));
+    if (p.dtype == ORTMI_F32)
+        hipLaunchKernelGGL((merge_kernel<true, PAGED>), units, dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((merge_kernel<false, PAGED>), units, dim3(256), 0, st, p);
     return check_launch("kv merge");
 }
 
@@ -306,10 +364,14 @@ extern "C" size_t ortmi_group_query_attention_quantized_workspace_size(
         return 0;
     size_t most = 0;  // over the types: fp32 has tiles of its own
     for (int dtype : {ORTMI_F32, ORTMI_F16}) {
-        int ntile, nsplit, chunk;
-        kvq::plan_slabs(batch, seq_len, num_heads, kv_num_heads, total_kv, dtype, ntile, nsplit,
-                        chunk);
-        most = std::max(most, kvq::ranges_bytes(batch * seq_len * num_heads, nsplit, head_size));
+        kvq::Params p{};
+        p.B = (int)batch;
+        p.S = (int)seq_len;
+        p.H = (int)num_heads;
+        p.KV = (int)kv_num_heads;
+        p.hd = (int)head_size;
+        p.dtype = dtype;
+        most = std::max(most, kvq::plan_slabs(p, total_kv, nullptr));
     }
     return most;
 }
@@ -330,7 +392,7 @@ extern "C" int ortmi_group_query_attention_quantized(
                               cache_type, dtype))
         return rc;
     ORTMI_REQUIRE(batch >= 0 && seq_len >= 0 && past_cap >= 0, what + ": negative size");
-    ORTMI_REQUIRE(batch * seq_len * num_heads < (1LL << 31) && past_cap + seq_len < (1LL << 31) &&
+    ORTMI_REQUIRE(batch * seq_len * num_heads < (1LL << 31) && past_cap + seq_len < (1LL << 31) - 4096 &&
                       batch * kv_num_heads < (1LL << 31),
                   what + ": too many rows");
     if (batch == 0 || seq_len == 0) return ORTMI_OK;
@@ -394,15 +456,11 @@ extern "C" int ortmi_group_query_attention_quantized(
     p.scale = (scale != 0.f ? scale : 1.0f / sqrtf((float)hd)) * 1.44269504088896341f;
     p.dtype = dtype;
     p.out = output;
-    kvq::plan_slabs(batch, seq_len, num_heads, kv_num_heads, vpast + seq_len, dtype, p.ntile,
-                    p.nsplit, p.chunk);
-    if (!kvq::tile_head(hd)) p.nsplit = 1;
-    const size_t need = kvq::ranges_bytes(batch * seq_len * num_heads, p.nsplit, hd);
+    const size_t need = kvq::plan_slabs(p, vpast + seq_len, static_cast<char*>(workspace));
     if (need && (!workspace || workspace_bytes < need))
         return fail(ORTMI_E_WORKSPACE, what + ": workspace too small");
     ORTMI_REQUIRE(!need || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                   what + ": workspace must be 16-byte aligned");
-    kvq::place_ranges(p, static_cast<char*>(workspace));
     const int64_t rb = kvq::row_bytes(p.code, (int)hd), slabs = batch * kv_num_heads;
     const int64_t kept = shared ? past_cap : vpast;  // rows of a past that is another buffer
     const void* past[2] = {past_key, past_value};
@@ -421,10 +479,19 @@ extern "C" size_t ortmi_paged_attention_quantized_workspace_size(
     if (num_tokens <= 0 || batch <= 0 || kv_num_heads <= 0 || num_heads < kv_num_heads ||
         !kvq::tile_head(head_size))
         return 0;
-    int nsplit, chunk;
-    kvq::plan_pages(batch, kv_num_heads, max_context, nsplit, chunk);
-    return kvq::ranges_bytes(num_tokens * num_heads, nsplit, head_size) +
-           (size_t)(kvq::max_page_tiles(num_tokens, batch, num_heads / kv_num_heads, 64) + 1) * 8;
+    size_t most = 0;  // over the types: fp32 has tiles of its own
+    for (int dtype : {ORTMI_F32, ORTMI_F16}) {
+        kvq::Params p{};
+        p.B = (int)batch;
+        p.T = (int)num_tokens;
+        p.H = (int)num_heads;
+        p.KV = (int)kv_num_heads;
+        p.hd = (int)head_size;
+        p.limit = (int)std::min<int64_t>(max_context, INT32_MAX);
+        p.dtype = dtype;
+        most = std::max(most, kvq::plan_pages(p, nullptr));
+    }
+    return most;
 }
 
 extern "C" int ortmi_paged_attention_quantized(
@@ -449,6 +516,8 @@ extern "C" int ortmi_paged_attention_quantized(
                   what + ": bad cache or batch shape");
     ORTMI_REQUIRE(max_context > 0, what + ": max_context must be positive");
     ORTMI_REQUIRE(num_tokens * num_heads + 64 * batch < (1LL << 31), what + ": too many rows");
+    ORTMI_REQUIRE(std::min<int64_t>(max_context, max_blocks * block_size) < (1LL << 31) - 4096,
+                  what + ": too many keys");
     if (num_tokens == 0) return ORTMI_OK;
     ORTMI_REQUIRE(query && key && value && key_cache && value_cache && cum_seqlens &&
                       past_seqlens && block_table && output,
@@ -473,7 +542,7 @@ extern "C" int ortmi_paged_attention_quantized(
     p.KV = (int)kv_num_heads;
     p.hd = (int)head_size;
     p.T = (int)num_tokens;
-    p.limit = (int)std::min<int64_t>({max_context, max_blocks * block_size, INT32_MAX});
+    p.limit = (int)std::min<int64_t>(max_context, max_blocks * block_size);
     p.cos = cos_cache;
     p.sin = sin_cache;
     p.half = (int)rotary_half;
@@ -490,26 +559,18 @@ extern "C" int ortmi_paged_attention_quantized(
     p.sink = head_sink;
     p.dtype = dtype;
     p.out = output;
-    p.blk_shift = -1;
-    for (int i = 0; i < 31; ++i)
-        if (block_size == 1LL << i) p.blk_shift = i;
+    if (const uint32_t d = (uint32_t)(block_size / 16)) {
+        p.blk_shift = 27;
+        while (p.blk_shift < 58 && (1u << (p.blk_shift - 27)) < d) ++p.blk_shift;
+        p.blk_mul = (uint32_t)(((1ULL << p.blk_shift) + d - 1) / d);
+    }
     p.nsplit = 1;
     if (kvq::tile_head(head_size)) {
-        kvq::plan_pages(batch, kv_num_heads, max_context, p.nsplit, p.chunk);
-        p.max_tiles = kvq::max_page_tiles(num_tokens, batch, num_heads / kv_num_heads,
-                                          kvq::prompt_width(dtype));
-        const size_t need = kvq::ranges_bytes(num_tokens * num_heads, p.nsplit, head_size) +
-                            (size_t)(p.max_tiles + 1) * 8;
+        const size_t need = kvq::plan_pages(p, static_cast<char*>(workspace));
         if (!workspace || workspace_bytes < need)
             return fail(ORTMI_E_WORKSPACE, what + ": workspace too small");
         ORTMI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                       what + ": workspace must be 16-byte aligned");
-        char* ws = kvq::place_ranges(p, static_cast<char*>(workspace));
-        p.tile_count = reinterpret_cast<int*>(ws);
-        p.tiles = reinterpret_cast<int2*>(ws + 8);
-        // Prompt tiles: ranges of four times the keys (their work fills the GPU sooner).
-        p.tile_chunk = (int)std::min<int64_t>(4LL * p.chunk, 1 << 23);
-        p.tile_nsplit = (p.nsplit + 3) / 4;
     }
     return kvq::attend<true>(p, as_stream(stream));
 }

@@ -29,6 +29,8 @@
 // first, which the registers (200 of 256 at two waves a SIMD) leave no other wave for.
 #pragma once
 
+#include <algorithm>
+
 #include "kvq.h"
 
 namespace ortmi {
@@ -186,11 +188,12 @@ struct Source {
     using L = Layout<CODE, HD>;
     const Params& p;
     const uint8_t *kbase, *vbase;
-    int b, k0, k1;
+    const int32_t* table;
+    int k0, k1;
     uint32_t stride, kat, kat2, vat, vat2;
 
-    __device__ __forceinline__ Source(const Params& p_, int b_, int h, int k0_, int k1_)
-        : p(p_), b(b_), k0(k0_), k1(k1_) {
+    __device__ __forceinline__ Source(const Params& p_, int b, int h, int k0_, int k1_)
+        : p(p_), table(p_.bt + (PAGED ? (int64_t)b * p_.maxb : 0)), k0(k0_), k1(k1_) {
         const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
         stride = (uint32_t)(PAGED ? p.KV * L::RB : L::RB);
         const int64_t at = (PAGED ? (int64_t)h : cache_row<false>(p, b, h, k0)) * L::RB;
@@ -201,17 +204,27 @@ struct Source {
         vat = 4 * q * stride + m * L::kValStep;
         vat2 = 4 * q * stride + m * (L::kValStep / 2);
     }
+    // Logical block of a key: key / blk, both in units of 16 (blk_mul is 2^blk_shift / (blk / 16),
+    // rounded up: exact for 27 bits).
+    __device__ __forceinline__ uint32_t logical(int key) const {
+        return (uint32_t)(((uint64_t)((uint32_t)key >> 4) * p.blk_mul) >> p.blk_shift);
+    }
+    // The block table's entry for the key tile at `key`, its last one behind the table's end: a
+    // load nothing waits for until the entry is used.
+    __device__ __forceinline__ int entry(int key) const {
+        if constexpr (!PAGED) return 0;
+        return table[min(logical(key), (uint32_t)p.maxb - 1)];
+    }
+    // Whether a key tile with this entry has no block.
+    __device__ __forceinline__ bool gone(int key, int id) const {
+        if constexpr (!PAGED) return false;
+        return (logical(key) >= (uint32_t)p.maxb) | ((uint32_t)id >= (uint32_t)p.nblk);
+    }
     // Slot of the key tile at `key`: -1 behind the end and where there is no block.
-    __device__ __forceinline__ int slot(int key) const {
-        int s = -1;
-        if constexpr (PAGED) {
-            if (key < k1) {
-                const int lb = p.blk_shift >= 0 ? key >> p.blk_shift : key / p.blk;
-                const int id = lb < p.maxb ? p.bt[(int64_t)b * p.maxb + lb] : -1;
-                s = id >= 0 && id < p.nblk ? id * p.blk + (key - lb * p.blk) : -1;
-            }
-        }
-        return s;
+    __device__ __forceinline__ int slot(int key, int id) const {
+        if constexpr (!PAGED) return -1;
+        const bool is = (key < k1) & !gone(key, id);
+        return is ? id * p.blk + (key - (int)logical(key) * p.blk) : -1;
     }
     // The resource of the cache rows of a tile in a page.
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t page(const uint8_t* base, int key, int slot) const {
@@ -248,7 +261,10 @@ struct Source {
             }
         }
     }
-    __device__ __forceinline__ int2 slots(int kb) const { return make_int2(slot(kb), slot(kb + 16)); }
+    __device__ __forceinline__ int2 ids(int kb) const { return make_int2(entry(kb), entry(kb + 16)); }
+    __device__ __forceinline__ int2 slots(int kb, int2 id) const {
+        return make_int2(slot(kb, id.x), slot(kb + 16, id.y));
+    }
     __device__ __forceinline__ void load(int kb, int2 sl, Block<CODE, HD>& o) const {
         keys(kb, sl.x, o.k[0]);
         keys(kb + 16, sl.y, o.k[1]);
@@ -259,29 +275,38 @@ struct Source {
 template <int HD>
 constexpr int kRowFloats = HD + 4;  // of a row in LDS: four more than a multiple of the banks
 
-// N consecutive elements of a 16-byte aligned row as fp32.
-template <int N, bool F32>
-__device__ __forceinline__ void load_piece(const void* base, int64_t at, int dtype, float (&x)[N]) {
-    if constexpr (F32) {
-        const float* s = static_cast<const float*>(base) + at;
+// Four consecutive elements of a row, 8-byte aligned (fp32: 16). Loads and conversions are
+// apart: the conversion's branch on the type would otherwise wait for each load before the next
+// is issued.
+template <bool F32>
+struct Piece {
+    std::conditional_t<F32, uint4, uint2> w;
+    __device__ __forceinline__ void load(const void* base, int64_t at) {
+        w = *reinterpret_cast<const decltype(w)*>(static_cast<const uint8_t*>(base) + at * (F32 ? 4 : 2));
+    }
+    template <bool HALF>
+    __device__ __forceinline__ float get(int i) const {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(&w);
+        if constexpr (F32) return __builtin_bit_cast(float, u[i]);
+        else if constexpr (HALF) return (float)as_half2(u[i / 2])[i & 1];
+        else return to_f32((uint16_t)(u[i / 2] >> (16 * (i & 1))));
+    }
+};
+// New rows are taken by groups of lanes, each with four channels of the first half of the row
+// and their partners in the rotation, four of the second: 8 lanes at head size 64, 16 at 128,
+// 12 of 16 at 96.
+template <int HD>
+constexpr int kRowLanes = HD == 64 ? 8 : 16;
+// N scales from element `at` on, or one.
+template <int N>
+__device__ __forceinline__ void load_scales(const float* base, bool chan, int at, float (&x)[N]) {
+    if (chan) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(s + i);
-            x[i] = v.x;
-            x[i + 1] = v.y;
-        }
+        for (int i = 0; i < N; ++i) x[i] = base[at + i];
     } else {
-        const uint32_t* s = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(base) + at);
-        uint32_t w[N / 2];
+        const float one = base[0];
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) w[i] = s[i];
-        if (dtype == ORTMI_F16) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = (float)as_half2(w[i / 2])[i & 1];
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = to_f32((uint16_t)(w[i / 2] >> (16 * (i & 1))));
-        }
+        for (int i = 0; i < N; ++i) x[i] = one;
     }
 }
 
@@ -292,96 +317,128 @@ __device__ __forceinline__ float load_one(const void* base, int64_t at, int dtyp
     return dtype == ORTMI_F16 ? (float)__builtin_bit_cast(half_t, u) : to_f32(u);
 }
 
-// The query rows of columns c0 .. c0 + GR NC - 1 into LDS, 16 lanes a column, each a sixteenth
-// of its channels: (normalised and) rotated, times the key scales, brought to [2^10, 2^11) and
-// rounded to fp16, in the order [column][k step][quarter][8] of the right operand (SPLIT: the
-// second halves behind). f: what a product is to be multiplied by; pos: the column's position,
-// -1 for none. The code is kept short: a workgroup runs it once, from a cold cache.
-template <int CODE, int HD, int GR, int NC, bool F32, bool SPLIT>
+// The query rows of columns c0 .. c0 + COLS - 1 into LDS: (normalised and) rotated, times the key
+// scales, brought to [2^10, 2^11) and rounded to fp16, in the order [column][k step][quarter][8]
+// of the right operand (SPLIT: the second halves behind). f: what a product is to be multiplied
+// by; pos: the column's position, -1 for none. Behind sq's rows is room for as many of fp32.
+template <int CODE, int HD, int COLS, int THREADS, bool F32, bool SPLIT>
 __device__ __forceinline__ void stage_queries(const Params& p, const Seq& s, int h, int c0,
                                               half_t* sq, float* f, int* pos) {
     using L = Layout<CODE, HD>;
-    constexpr int N = HD / 16;
-    const int G = p.H / p.KV, tid = threadIdx.x, lane = tid & 15, group = tid >> 4;
-    const int ch = lane * N;
-    const bool second = ch >= HD / 2;
-    const int other = second ? ch - HD / 2 : ch + HD / 2;
-    float x[NC][N], o[NC][N], co[NC][N], si[NC][N];
-#pragma unroll
-    for (int cc = 0; cc < NC; ++cc) {
-        const int c = GR * cc + group, r = (c0 + c) / G, g = (c0 + c) - r * G;
-        const bool live = r < s.real;
-        const int tok = s.tok0 + (live ? r : 0), at = s.past + (live ? r : 0);
-        const int64_t x0 = (int64_t)tok * p.q_tok + (int64_t)(h * G + g) * HD;
-        load_piece<N, F32>(p.q, x0 + ch, p.dtype, x[cc]);
-        if (p.cos && p.pieces) {
-            const int64_t k = min((int64_t)at, p.max_pos - 1) * (HD / 2) + (second ? other : ch);
-            load_piece<N, F32>(p.q, x0 + other, p.dtype, o[cc]);
-            load_piece<N, F32>(p.cos, k, p.dtype, co[cc]);
-            load_piece<N, F32>(p.sin, k, p.dtype, si[cc]);
-        }
-        if (lane == 0) pos[c] = live ? at : -1;
+    constexpr int W = kRowLanes<HD>, GR = std::min(COLS, THREADS / W), NC = COLS / GR;
+    const int G = p.H / p.KV, lane = threadIdx.x % W;
+    const int group = min((int)threadIdx.x / W, GR - 1);
+    const bool on = lane < HD / 8 && (int)threadIdx.x < GR * W;
+    const int ch = lane < HD / 8 ? 4 * lane : 0, hi = ch + HD / 2;
+    Piece<F32> x0[NC], x1[NC], co[NC], si[NC], w0, w1;
+    const bool rope = p.cos && p.pieces;
+    if (p.qw && p.pieces) {
+        w0.load(p.qw, ch);
+        w1.load(p.qw, hi);
     }
-    float sc[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) sc[i] = p.ks[p.k_chan ? h * HD + ch + i : 0];
+    float s0[4], s1[4];
+    load_scales<4>(p.ks, p.k_chan, h * HD + ch, s0);
+    load_scales<4>(p.ks, p.k_chan, h * HD + hi, s1);
+    // Column GR cc + group is head g of the group, row r; -1: a row that does not exist.
+    int g = (c0 + group) % G, r = (c0 + group) / G;
+    const int dg = GR % G, dr = GR / G;
+    int64_t from[NC];
+    int at[NC];
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
-        const int c = GR * cc + group, r = (c0 + c) / G, g = (c0 + c) - r * G;
-        const bool live = r < s.real;
-        float rinv = 1.f;
-        if (p.qw) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) ss += x[cc][i] * x[cc][i];
-            rinv = 1.f / sqrtf(group_sum<16>(ss) / (float)HD + p.eps);
+        const int row = r < s.real ? r : 0;
+        at[cc] = s.past + row;
+        from[cc] = (int64_t)(s.tok0 + row) * p.q_tok + (int64_t)(h * G + g) * HD;
+        x0[cc].load(p.q, from[cc] + ch);
+        x1[cc].load(p.q, from[cc] + hi);
+        if (rope) {
+            const int64_t k = min((int64_t)at[cc], p.max_pos - 1) * (HD / 2) + ch;
+            co[cc].load(p.cos, k);
+            si[cc].load(p.sin, k);
         }
-        if (p.pieces) {
+        if (r >= s.real) at[cc] = -1;
+        r += dr;
+        g += dg;
+        if (g >= G) {
+            g -= G;
+            ++r;
+        }
+    }
+    auto stage = [&](auto half) {
+        constexpr bool HALF = decltype(half)::value;
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc) {
+            const int c = GR * cc + group;
+            float x[8], rinv = 1.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = x0[cc].template get<HALF>(i);
+                x[4 + i] = x1[cc].template get<HALF>(i);
+            }
             if (p.qw) {
-                float w[N];
-                load_piece<N, F32>(p.qw, ch, p.dtype, w);
+                float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < N; ++i) x[cc][i] = x[cc][i] * rinv * w[i];
-                if (p.cos) {
-                    load_piece<N, F32>(p.qw, other, p.dtype, w);
+                for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+                ss = group_sum<W>(lane < HD / 8 ? ss : 0.f);
+                rinv = 1.f / sqrtf(ss / (float)HD + p.eps);
+            }
+            if (p.pieces) {
+                if (p.qw) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) o[cc][i] = o[cc][i] * rinv * w[i];
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = x[i] * rinv * w0.template get<HALF>(i);
+                        x[4 + i] = x[4 + i] * rinv * w1.template get<HALF>(i);
+                    }
+                }
+                if (rope) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float a = x[i], b = x[4 + i];
+                        const float cv = co[cc].template get<HALF>(i), sv = si[cc].template get<HALF>(i);
+                        x[i] = a * cv - b * sv;
+                        x[4 + i] = b * cv + a * sv;
+                    }
+                }
+            } else if (on) {  // any rotation: element by element, by way of LDS (a register has no index)
+                const int64_t prow = min((int64_t)max(at[cc], 0), p.max_pos - 1) * p.half;
+                float* own = reinterpret_cast<float*>(sq + (SPLIT ? 2 : 1) * COLS * HD) + c * HD + 8 * lane;
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i)
+                    own[i] = query_elem(p, from[cc], prow, rinv, (i < 4 ? ch : hi - 4) + i);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = own[i];
+            }
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] *= i < 4 ? s0[i] : s1[i - 4];
+                top = fmaxf(top, fabsf(x[i]));
+            }
+            top = group_max<W>(top);
+            // A row of zeros, or with an infinity, is taken as it is.
+            const int ex = top > 0.f && top < INFINITY ? max(-100, min(ilogbf(top), 116)) : 10;
+            if (on) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    half_t* to = sq + c * HD + L::key_slot(b ? hi : ch);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float z = at[cc] >= 0 ? ldexpf(x[4 * b + i], 10 - ex) : 0.f;
+                        const half_t y = (half_t)z;
+                        constexpr int kStep = CODE == kInt4 ? 2 : 1;
+                        to[kStep * i] = y;
+                        if constexpr (SPLIT) to[COLS * HD + kStep * i] = (half_t)(z - (float)y);
+                    }
+                }
+                if (lane == 0) {
+                    f[c] = ldexpf(p.scale, ex - 10);
+                    pos[c] = at[cc];
                 }
             }
-            if (p.cos) {
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    x[cc][i] = x[cc][i] * co[cc][i] + (second ? o[cc][i] : -o[cc][i]) * si[cc][i];
-            }
-        } else {  // any rotation: element by element
-            const int at = s.past + (live ? r : 0);
-            const int64_t x0 = (int64_t)(s.tok0 + (live ? r : 0)) * p.q_tok + (int64_t)(h * G + g) * HD;
-            const int64_t prow = min((int64_t)at, p.max_pos - 1) * p.half;
-            for (int i = 0; i < N; ++i) {
-                const float v = query_elem(p, x0, prow, rinv, ch + i);
-#pragma unroll
-                for (int j = 0; j < N; ++j) x[cc][j] = j == i ? v : x[cc][j];
-            }
         }
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            x[cc][i] *= sc[i];
-            top = fmaxf(top, fabsf(x[cc][i]));
-        }
-        top = group_max<16>(top);
-        // A row of zeros, or with an infinity, is taken as it is.
-        const int ex = top > 0.f && top < INFINITY ? max(-100, min(ilogbf(top), 116)) : 10;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float z = live ? ldexpf(x[cc][i], 10 - ex) : 0.f;
-            const half_t hi = (half_t)z;
-            const int at = c * HD + L::key_slot(ch + i);
-            sq[at] = hi;
-            if constexpr (SPLIT) sq[GR * NC * HD + at] = (half_t)(z - (float)hi);
-        }
-        if (lane == 0) f[c] = ldexpf(p.scale, ex - 10);
-    }
+    };
+    if (F32 || p.dtype == ORTMI_F16) stage(std::true_type{});
+    else stage(std::false_type{});
     __syncthreads();
 }
 
@@ -457,6 +514,17 @@ __device__ __forceinline__ float output_factor(const Params& p, int head, float 
     return l != 0.f ? a / l : 0.f;
 }
 
+// One unit: a range of keys [k0, k1), `split` of `n`, for the tile of columns c0 .. of sequence
+// b and kv head h. The tile's units are first, first + step, ... in part and ml.
+struct Unit {
+    int b, h, c0, split, n, k0, k1, step;
+    int64_t first;
+    float *part, *ml;
+    __device__ __forceinline__ int64_t row(int i, int cols, int c) const {
+        return (first + (int64_t)i * step) * cols + c;
+    }
+};
+
 // N (2, 4 or 8) neighbouring channels of an output row, times their value scales vs; a factor
 // of 0 gives zeros whatever they are.
 template <int N, bool F32>
@@ -488,10 +556,33 @@ __device__ __forceinline__ void store_piece(const Params& p, int64_t at, const f
         else *reinterpret_cast<uint32_t*>(o) = w[0];
     }
 }
-template <int N>
-__device__ __forceinline__ void value_scales(const Params& p, int at, float (&vs)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) vs[j] = p.vs[p.v_chan ? at + j : 0];
+// A unit's columns from LDS rows, eight channels a thread and step, all of a row side by side:
+// as output times inv, or (one range of several) unscaled into part. Padded rows are zeros.
+// The scales are on their way while the rows are written: this waits for the other threads.
+template <int HD, bool F32, int COLS, int THREADS>
+__device__ __forceinline__ void write_rows(const Params& p, const Seq& s, const Unit& un,
+                                           const float* rows, const float* inv, int part_cols) {
+    constexpr int kPieces = HD / 8, kRows = THREADS / kPieces;
+    const int G = p.H / p.KV, ch = 8 * (threadIdx.x % kPieces);
+    float vs[8];
+    load_scales<8>(p.vs, p.v_chan, un.h * HD + ch, vs);
+    __syncthreads();
+#pragma unroll 1
+    for (int c = threadIdx.x / kPieces; c < COLS; c += kRows) {
+        const int r = (un.c0 + c) / G;
+        if (r >= s.rows || threadIdx.x >= kRows * kPieces) break;
+        const float* x = rows + c * kRowFloats<HD> + ch;
+        const float4_t a = *reinterpret_cast<const float4_t*>(x), b = *reinterpret_cast<const float4_t*>(x + 4);
+        if (un.n > 1 && r < s.real) {
+            float* o = un.part + un.row(un.split, part_cols, c) * HD + ch;
+            *reinterpret_cast<float4_t*>(o) = a;
+            *reinterpret_cast<float4_t*>(o + 4) = b;
+        } else if (un.n <= 1 || un.split == 0) {
+            const int64_t row = (int64_t)(s.tok0 + r) * p.H + un.h * G + (un.c0 + c - r * G);
+            const float y[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            store_piece<8, F32>(p, row * HD + ch, y, vs, r < s.real ? inv[c] : 0.f);
+        }
+    }
 }
 
 // ----------------------------------------------------------------- token tiles --
@@ -507,10 +598,11 @@ struct TokenShared {
     float m[4][16], l[4][16];
 };
 
-// One tile of columns 0 .. 15 over keys [k0, k1) of sequence s: range `split` of `nsplit`.
+// A unit of columns 0 .. 15 of sequence s.
 template <int CODE, int HD, bool F32, bool PAGED>
-__device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b, int h, int k0,
-                                           int k1, int split, int nsplit, TokenShared<HD, F32>& sh) {
+__device__ __forceinline__ void token_tile(const Params& p, const Seq& s, const Unit& un,
+                                           TokenShared<HD, F32>& sh) {
+    const int b = un.b, h = un.h, k0 = un.k0, k1 = un.k1;
     using L = Layout<CODE, HD>;
     constexpr int KS = L::KS, MT = L::MT;
     const int lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
@@ -520,10 +612,10 @@ __device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b,
     // The first block's rows are on their way while the queries are staged.
     const Source<CODE, HD, PAGED> src(p, b, h, k0, k1);
     int kb = k0 + 32 * wave;
-    int2 sl = src.slots(kb), sl_n = src.slots(kb + 128);
+    int2 id = src.ids(kb), id_n = src.ids(kb + 128), sl = src.slots(kb, id);
     Block<CODE, HD> cur, nxt;
     if (kb < k1) src.load(kb, sl, cur);
-    stage_queries<CODE, HD, 16, 1, F32, true>(p, s, h, 0, sh.queries, sh.f, sh.pos);
+    stage_queries<CODE, HD, 16, 256, F32, true>(p, s, h, 0, sh.queries, sh.f, sh.pos);
     const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries);
     half8_t Q[KS], QL[KS];
 #pragma unroll
@@ -542,9 +634,9 @@ __device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b,
     for (; kb < k1; kb += 128) {
         const int2 sl_c = sl;
         if (kb + 128 < k1) {
-            src.load(kb + 128, sl_n, nxt);
-            sl = sl_n;
-            sl_n = src.slots(kb + 256);
+            sl = src.slots(kb + 128, id_n);
+            id_n = src.ids(kb + 256);
+            src.load(kb + 128, sl, nxt);
         }
         float x[2][4];
 #pragma unroll
@@ -625,31 +717,13 @@ __device__ __forceinline__ void token_tile(const Params& p, const Seq& s, int b,
             for (int i = 0; i < 4; ++i) row[L::value_channel(4 * q + i, d)] = O[d][i];
         const int r = n / G, head = h * G + (n - r * G);
         if (q == 0 && r < s.real) {
-            const int64_t orow = (int64_t)(s.tok0 + r) * p.H + head;
-            if (nsplit > 1) {
-                p.ml[(orow * p.nsplit + split) * 2] = mm;
-                p.ml[(orow * p.nsplit + split) * 2 + 1] = sum;
-            } else {
+            if (un.n > 1)
+                reinterpret_cast<float2*>(un.ml)[un.row(un.split, p.tcols, n)] = make_float2(mm, sum);
+            else
                 sh.inv[n] = output_factor<F32, PAGED>(p, head, mm, sum);
-            }
         }
     }
-    __syncthreads();
-    constexpr int kPieces = HD / 4;  // of a row: four channels a thread and step
-    for (int i = threadIdx.x; i < 16 * kPieces; i += 256) {
-        const int c = i / kPieces, ch = 4 * (i % kPieces), r = c / G;
-        if (r >= s.rows) break;
-        const int64_t orow = (int64_t)(s.tok0 + r) * p.H + h * G + (c - r * G);
-        const float4_t v = *reinterpret_cast<const float4_t*>(sh.rows + c * kRowFloats<HD> + ch);
-        if (nsplit > 1 && r < s.real) {
-            *reinterpret_cast<float4_t*>(p.part + (orow * p.nsplit + split) * HD + ch) = v;
-        } else if (nsplit <= 1 || split == 0) {
-            const float y[4] = {v[0], v[1], v[2], v[3]};
-            float vs[4];
-            value_scales(p, h * HD + ch, vs);
-            store_piece<4, F32>(p, orow * HD + ch, y, vs, r < s.real ? sh.inv[c] : 0.f);
-        }
-    }
+    write_rows<HD, F32, 16, 256>(p, s, un, sh.rows, sh.inv, p.tcols);
 }
 
 // ---------------------------------------------------------------- prompt tiles --
@@ -662,17 +736,20 @@ struct PromptShared {
     union {
         __align__(16) half_t queries[(F32 ? 2 : 1) * kCols * HD];
         Blocks team[2];
-        __align__(16) float4_t out[4][HD / 16][kNT][64];  // the second team's outputs
+        struct {
+            __align__(16) float4_t out[4][HD / 16][kNT][64];  // the second team's outputs
+            __align__(16) float rows[kCols * kRowFloats<HD>];  // the tile's
+        };
     };
-    float f[kCols], m[kCols], l[kCols];
+    float f[kCols], m[kCols], l[kCols], inv[kCols];
     int pos[kCols];
 };
 
-// One tile of columns c0 .. over keys [k0, k1) of sequence s: range `split` of `nsplit`.
+// A unit of columns c0 .. c0 + 127 (fp32: 63) of sequence s.
 template <int CODE, int HD, bool F32, bool PAGED>
-__device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b, int h, int c0,
-                                            int k0, int k1, int split, int nsplit,
+__device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, const Unit& un,
                                             PromptShared<CODE, HD, F32>& sh) {
+    const int b = un.b, h = un.h, c0 = un.c0, k0 = un.k0, k1 = un.k1;
     using L = Layout<CODE, HD>;
     using SH = PromptShared<CODE, HD, F32>;
     constexpr int KS = L::KS, MT = L::MT, NT = SH::kNT, UH = (MT / 2 + 1) / 2;
@@ -685,16 +762,22 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
     // Of a block at kb a wave decodes key tile `wave`, and of the values of its half of the
     // keys (wave / 2) half of the channel tiles.
     uint32_t rk[L::KW], rv[8][L::VW];
-    int slot[4], slot_n[4];
-    auto slots = [&](int kb, int (&sl)[4]) {
+    // Entries of the block of keys to be loaded next, and the key tiles without a block (bits) of
+    // this one and the next.
+    int id[4];
+    uint32_t gone = 0, gone_n = 0;
+    auto ids = [&](int kb) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) sl[t] = src.slot(kb + 16 * t);
+        for (int t = 0; t < 4; ++t) id[t] = src.entry(kb + 16 * t);
     };
-    auto load = [&](int kb, const int (&sl)[4]) {
-        const int s0 = sl[0], s1 = sl[1], s2 = sl[2], s3 = sl[3];
-        const int a = wave & 2 ? s2 : s0, c = wave & 2 ? s3 : s1;
+    auto load = [&](int kb) {
+        gone_n = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) gone_n |= (uint32_t)src.gone(kb + 16 * t, id[t]) << t;
+        const int a0 = id[0], a1 = id[1], a2 = id[2], a3 = id[3], kv = kb + 32 * (wave >> 1);
+        const int a = src.slot(kv, wave & 2 ? a2 : a0), c = src.slot(kv + 16, wave & 2 ? a3 : a1);
         src.keys(kb + 16 * wave, wave & 1 ? c : a, rk);
-        src.values(kb + 32 * (wave >> 1), a, c, rv);
+        src.values(kv, a, c, rv);
     };
     auto decode = [&](int buf) {
 #pragma unroll
@@ -710,9 +793,10 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
     };
 
     int kb = k0 + 64 * team;
-    slots(kb, slot);
-    if (kb < k1) load(kb, slot);
-    stage_queries<CODE, HD, 32, 2 * NT, F32, F32>(p, s, h, c0, sh.queries, sh.f, sh.pos);
+    ids(kb);
+    if (kb < k1) load(kb);
+    ids(kb + 128);
+    stage_queries<CODE, HD, SH::kCols, 512, F32, F32>(p, s, h, c0, sh.queries, sh.f, sh.pos);
     const half8_t* sq = reinterpret_cast<const half8_t*>(sh.queries);
     half8_t Q[NT][KS], QL[F32 ? NT : 1][KS];
     float f[NT];
@@ -744,18 +828,18 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
     }
     __syncthreads();  // the queries are read: the blocks take their place
     if (kb < k1) decode(0);
-    slots(kb + 128, slot_n);
-    if (kb + 128 < k1) load(kb + 128, slot_n);
+    gone = gone_n;
+    if (kb + 128 < k1) load(kb + 128);
+    ids(kb + 256);
     __syncthreads();
     int buf = 0;
     for (int first_kb = k0; first_kb < k1; first_kb += 128, kb += 128, buf ^= 1) {
-        const int sl[4] = {slot[0], slot[1], slot[2], slot[3]};
+        const uint32_t out = gone;
         if (kb + 128 < k1) {
             decode(buf ^ 1);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) slot[t] = slot_n[t];
-            slots(kb + 256, slot_n);
-            if (kb + 256 < k1) load(kb + 256, slot_n);
+            gone = gone_n;
+            if (kb + 256 < k1) load(kb + 256);
+            ids(kb + 384);
         }
         if (kb <= last && kb < k1) {
             float x[NT][4][4];
@@ -778,14 +862,13 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[t][t4][i] = S[t][i] * f[t];
             }
-            const bool gone = PAGED && (sl[0] < 0 || sl[1] < 0 || sl[2] < 0 || sl[3] < 0);
-            if (kb + 63 > first || kb + 64 > k1 || gone) {
+            if (kb + 63 > first || kb + 64 > k1 || (PAGED && out)) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int t4 = 0; t4 < 4; ++t4)
                         mask_scores(x[t][t4], kb + 16 * t4,
-                                    PAGED && sl[t4] < 0 ? -1 : min(pos[t], k1 - 1));
+                                    PAGED && (out >> t4 & 1) ? -1 : min(pos[t], k1 - 1));
             }
             bool grow = false;
             float top[NT];
@@ -825,8 +908,7 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
         __syncthreads();
     }
 
-    // The second team's outputs to the first, which writes them: a lane's neighbouring channels
-    // at once.
+    // The second team's outputs to the first, which adds its own.
     if (team) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -840,133 +922,118 @@ __device__ __forceinline__ void prompt_tile(const Params& p, const Seq& s, int b
         }
     }
     __syncthreads();
-    if (team) return;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const float m1 = sh.m[cw + 16 * t + n], mm = fmaxf(m[t], m1);
-        const float a0 = __builtin_amdgcn_exp2f(m[t] - mm), a1 = __builtin_amdgcn_exp2f(m1 - mm);
-        m[t] = mm;
-        l[t] = quarters_sum(l[t]) * a0 + sh.l[cw + 16 * t + n] * a1;
-#pragma unroll
-        for (int d = 0; d < MT; ++d) O[d][t] = O[d][t] * a0 + sh.out[wave][d][t][lane] * a1;
-    }
-    constexpr int W = HD == 128 ? 8 : 4;  // (HD 96: and two of the last third)
-    int64_t row[NT];
-    float inv[NT];
-    bool live[NT], partial[NT], any[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int c = c0 + cw + 16 * t + n, r = c / G, head = h * G + (c - r * G);
-        row[t] = (int64_t)(s.tok0 + r) * p.H + head;
-        live[t] = r < s.real;
-        partial[t] = nsplit > 1 && live[t];
-        any[t] = r < s.rows && (live[t] || nsplit <= 1 || split == 0);
-        if (partial[t] && q == 0) {
-            p.ml[(row[t] * p.nsplit + split) * 2] = m[t];
-            p.ml[(row[t] * p.nsplit + split) * 2 + 1] = l[t];
-        }
-        inv[t] = live[t] ? output_factor<F32, PAGED>(p, head, m[t], l[t]) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int ch = L::value_channel(4 * q + i, 0), ch2 = L::value_channel(4 * q + i, MT - 2);
-        float vs[W], vs2[2];
-        value_scales(p, h * HD + ch, vs);
-        if constexpr (HD == 96) value_scales(p, h * HD + ch2, vs2);
+    if (!team) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if (!any[t]) continue;
-            float v[W];
+            const int c = cw + 16 * t + n, r = (c0 + c) / G;
+            const float m1 = sh.m[c], mm = fmaxf(m[t], m1);
+            const float a0 = __builtin_amdgcn_exp2f(m[t] - mm), a1 = __builtin_amdgcn_exp2f(m1 - mm);
+            const float sum = quarters_sum(l[t]) * a0 + sh.l[c] * a1;
+            float* row = sh.rows + c * kRowFloats<HD>;
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[j] = O[j][t][i];
-            const float z[2] = {O[MT - 2][t][i], O[MT - 1][t][i]};
-            if (partial[t]) {
-                float* part = p.part + (row[t] * p.nsplit + split) * HD;
+            for (int d = 0; d < MT; ++d) O[d][t] = O[d][t] * a0 + sh.out[wave][d][t][lane] * a1;
 #pragma unroll
-                for (int j = 0; j < W; j += 4)
-                    *reinterpret_cast<float4_t*>(part + ch + j) = float4_t{v[j], v[j + 1], v[j + 2], v[j + 3]};
+            for (int i = 0; i < 4; ++i) {  // a lane's neighbouring channels at once
+                const int ch = L::value_channel(4 * q + i, 0);
+#pragma unroll
+                for (int d = 0; d < (HD == 96 ? 4 : MT); d += 4)
+                    *reinterpret_cast<float4_t*>(row + ch + d) =
+                        float4_t{O[d][t][i], O[d + 1][t][i], O[d + 2][t][i], O[d + 3][t][i]};
                 if constexpr (HD == 96)
-                    *reinterpret_cast<float2*>(part + ch2) = make_float2(z[0], z[1]);
-            } else {
-                store_piece<W, F32>(p, row[t] * HD + ch, v, vs, inv[t]);
-                if constexpr (HD == 96) store_piece<2, F32>(p, row[t] * HD + ch2, z, vs2, inv[t]);
+                    *reinterpret_cast<float2*>(row + L::value_channel(4 * q + i, 4)) =
+                        make_float2(O[4][t][i], O[5][t][i]);
+            }
+            if (q == 0 && r < s.real) {
+                if (un.n > 1)
+                    reinterpret_cast<float2*>(un.ml)[un.row(un.split, SH::kCols, c)] = make_float2(mm, sum);
+                else
+                    sh.inv[c] = output_factor<F32, PAGED>(p, h * G + (c0 + c - r * G), mm, sum);
             }
         }
     }
+    write_rows<HD, F32, SH::kCols, 512>(p, s, un, sh.rows, sh.inv, SH::kCols);
 }
 
 // -------------------------------------------------------------------- new rows --
-// append_row in pieces: 16 lanes a row, each a sixteenth of its channels, which lie side by
-// side as their partners in the rotation do.
+// append_row in pieces.
 template <int CODE, int HD, bool F32, bool PAGED>
 __device__ __forceinline__ void append_piece(const Params& p, int b, const Seq& s, int r, int h,
                                              bool is_v, int lane) {
-    constexpr int N = HD / 16, RB = row_bytes(CODE, HD);
-    const int pos = s.past + r, c0 = lane * N;
+    constexpr int RB = row_bytes(CODE, HD);
+    const int pos = s.past + r, c0 = lane < HD / 8 ? 4 * lane : 0, c1 = c0 + HD / 2;
     const int64_t row = cache_row<PAGED>(p, b, h, pos);
-    const int64_t x0 = (int64_t)(s.tok0 + r) * p.kv_tok + (int64_t)h * HD;
+    const int64_t from = (int64_t)(s.tok0 + r) * p.kv_tok + (int64_t)h * HD;
     const void* src = is_v ? p.v : p.k;
-    const bool rope = !is_v && p.cos, second = c0 >= HD / 2;
-    float x[N], o[N], co[N], si[N], w[N], wo[N];
-    load_piece<N, F32>(src, x0 + c0, p.dtype, x);
-    const int c1 = second ? c0 - HD / 2 : c0 + HD / 2;  // of the partners
+    const bool rope = !is_v && p.cos, norm = p.kw && !is_v;
+    Piece<F32> x0, x1, co, si, w0, w1;
+    float sc[2][4];
+    x0.load(src, from + c0);
+    x1.load(src, from + c1);
+    load_scales<4>(is_v ? p.vs : p.ks, is_v ? p.v_chan : p.k_chan, h * HD + c0, sc[0]);
+    load_scales<4>(is_v ? p.vs : p.ks, is_v ? p.v_chan : p.k_chan, h * HD + c1, sc[1]);
     if (rope) {
-        const int64_t at = min((int64_t)pos, p.max_pos - 1) * (HD / 2) + (second ? c1 : c0);
-        load_piece<N, F32>(src, x0 + c1, p.dtype, o);
-        load_piece<N, F32>(p.cos, at, p.dtype, co);
-        load_piece<N, F32>(p.sin, at, p.dtype, si);
+        const int64_t at = min((int64_t)pos, p.max_pos - 1) * (HD / 2) + c0;
+        co.load(p.cos, at);
+        si.load(p.sin, at);
     }
-    double rinv = 1.0;
-    const bool norm = p.kw && !is_v;
-    if (p.kw) {  // (a value row's lanes go along)
-        double ss = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss += (double)x[i] * (double)x[i];
-#pragma unroll
-        for (int k = 8; k; k >>= 1) ss += __shfl_xor(ss, k, 64);
-        rinv = 1.0 / sqrt(ss / HD + (double)p.eps);
-        load_piece<N, F32>(p.kw, c0, p.dtype, w);
-        load_piece<N, F32>(p.kw, c1, p.dtype, wo);
+    if (p.kw) {
+        w0.load(p.kw, c0);
+        w1.load(p.kw, c1);
     }
-    if (row < 0) return;
-    const float* sc = (is_v ? p.vs : p.ks);
-    const bool chan = is_v ? p.v_chan : p.k_chan;
-    uint32_t u[N];
+    auto codes = [&](auto half) {
+        constexpr bool HALF = decltype(half)::value;
+        double x[2][4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        double a = x[i];
-        if (norm) a = a * rinv * (double)w[i];
-        if (rope) {
-            double e = o[i];
-            if (norm) e = e * rinv * (double)wo[i];
-            const double f = a * (double)co[i], g = e * (double)si[i];
-            a = second ? f + g : f - g;
+        for (int i = 0; i < 4; ++i) {
+            x[0][i] = x0.template get<HALF>(i);
+            x[1][i] = x1.template get<HALF>(i);
         }
-        u[i] = encode(a, sc[chan ? h * HD + c0 + i : 0], CODE);
-    }
-    uint8_t* dst = (is_v ? p.vc : p.kc) + row * RB + (CODE == kInt4 ? c0 / 2 : c0);
-    if constexpr (CODE == kInt4) {
-        uint32_t v = 0;
+        if (p.kw) {  // (a value row's lanes go along)
+            double ss = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v |= u[i] << (4 * i);
-        if constexpr (N == 8) *reinterpret_cast<uint32_t*>(dst) = v;
-        else if constexpr (N == 4) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)v;
-        else
+            for (int i = 0; i < 4; ++i) ss += x[0][i] * x[0][i] + x[1][i] * x[1][i];
+            ss = lane < HD / 8 ? ss : 0.0;
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) dst[i] = (uint8_t)(v >> (8 * i));
-    } else {
+            for (int k = kRowLanes<HD> / 2; k; k >>= 1) ss += __shfl_xor(ss, k, 64);
+            const double rinv = norm ? 1.0 / sqrt(ss / HD + (double)p.eps) : 1.0;
 #pragma unroll
-        for (int i = 0; i < N; i += 2)
-            *reinterpret_cast<uint16_t*>(dst + i) = (uint16_t)(u[i] | (u[i + 1] << 8));
-    }
+            for (int i = 0; i < 4; ++i) {
+                x[0][i] = norm ? x[0][i] * rinv * (double)w0.template get<HALF>(i) : x[0][i];
+                x[1][i] = norm ? x[1][i] * rinv * (double)w1.template get<HALF>(i) : x[1][i];
+            }
+        }
+        if (row < 0 || lane >= HD / 8) return;
+        uint8_t* dst = (is_v ? p.vc : p.kc) + row * RB;
+        if (rope) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const double a = x[0][i], e = x[1][i];
+                const double c = co.template get<HALF>(i), d = si.template get<HALF>(i);
+                x[0][i] = a * c - e * d;
+                x[1][i] = e * c + a * d;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint32_t u = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                u |= encode(x[j][i], sc[j][i], CODE) << ((CODE == kInt4 ? 4 : 8) * i);
+            const int ch = j ? c1 : c0;
+            if constexpr (CODE == kInt4) *reinterpret_cast<uint16_t*>(dst + ch / 2) = (uint16_t)u;
+            else *reinterpret_cast<uint32_t*>(dst + ch) = u;
+        }
+    };
+    if (F32 || p.dtype == ORTMI_F16) codes(std::true_type{});
+    else codes(std::false_type{});
 }
 
 // Rows r0 .. r1 - 1 of sequence s, key and value of one kv head, by the workgroup.
 template <int CODE, int HD, bool F32, bool PAGED>
 __device__ __forceinline__ void append_rows(const Params& p, int b, const Seq& s, int r0, int r1,
                                             int h) {
-    const int lane = threadIdx.x & 15;
-    for (int i = 2 * r0 + (int)(threadIdx.x >> 4); i < 2 * r1; i += (int)(blockDim.x >> 4)) {
+    const int w = p.pieces ? kRowLanes<HD> : 16, lane = threadIdx.x % w;
+    for (int i = 2 * r0 + (int)threadIdx.x / w; i < 2 * r1; i += (int)blockDim.x / w) {
         if (p.pieces) append_piece<CODE, HD, F32, PAGED>(p, b, s, i >> 1, h, i & 1, lane);
         else append_row<PAGED>(p, b, s, i >> 1, h, i & 1, lane);
     }
@@ -985,39 +1052,188 @@ __device__ __forceinline__ bool sequence_of_token(const Params& p, int tok, int&
     return tok >= s.tok0 && tok < s.tok0 + s.rows;
 }
 
-// The prompt tiles of the sequences with more than 16 columns, in order, by one wave. Ranges
-// of tokens are clamped to the call's (sequence()), and at most max_tiles are written.
-__device__ __forceinline__ void list_tiles(const Params& p) {
-    const int lane = threadIdx.x & 63, G = p.H / p.KV, w = prompt_width(p.dtype);
-    int base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int b = b0 + lane;
-        const int cols = b < p.B ? sequence<true>(p, b).rows * G : 0;
-        const int n = cols > 16 ? (cols + w - 1) / w : 0;
-        int incl = n;
+// Keys of a range where `total` keys are to be taken in about `items` ranges.
+constexpr int kMostKeys = 1 << 24;  // a range's bytes stay below 2^32
+__device__ __forceinline__ int range_keys(int64_t total, int items, int least) {
+    const int64_t per = (total / items + 128) & ~127LL;  // above total / items
+    return (int)max((int64_t)least, min(per, (int64_t)kMostKeys));
+}
+// Units that n of a sequence's ranges put into part and ml: with one range, none.
+__device__ __forceinline__ int64_t parts_of(int64_t n, int64_t tiles) { return n > 1 ? n * tiles : 0; }
+
+__device__ __forceinline__ int64_t scan64(int64_t x, int lane) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += v;
-        }
-        const int first = base + incl - n;
-        for (int i = 0; i < n && first + i < p.max_tiles; ++i) p.tiles[first + i] = make_int2(b, w * i);
-        base += __shfl(incl, 63, 64);
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t v = __shfl_up(x, o, 64);
+        x += lane >= o ? v : 0;
     }
-    if (lane == 0) *p.tile_count = min(base, p.max_tiles);
+    return x;
 }
 
-// New keys and values into the cache: 16 lanes per (token, kv head, key or value). Pages: the
-// first workgroup lists the tiles.
+// Pages: the ranges, by one wave. Token tiles are those of sequences with at most 16 columns;
+// the others have prompt tiles, all over the ranges of the sequence's last. plan[b]: the units
+// (over KV) in front of sequence b, of token tiles x (in part: y), of prompt tiles z (in ppart:
+// w); plan[B]: all units x, z and the keys of a range y, w. Ranges of equal size, whatever the
+// sequences' lengths, keep the GPU evenly filled. Ranges that are not their tile's only one are
+// at most twice the units aimed at: n ranges of c keys, n > 1, lie over more than n c / 2 keys.
+template <bool F32>
+__device__ __forceinline__ void plan_units(const Params& p) {
+    constexpr int kW = prompt_width(F32 ? ORTMI_F32 : ORTMI_F16);
+    const int lane = threadIdx.x & 63, G = p.H / p.KV;
+    int64_t total[2] = {0, 0};
+    auto shape = [&](int b, int& kend, int& tiles) {
+        kend = tiles = 0;
+        if (b >= p.B) return;
+        const Seq s = sequence<true>(p, b);
+        const int64_t cols = (int64_t)s.rows * G;
+        if (s.rows > 0) kend = s.keys_to(s.rows - 1, p.limit);
+        tiles = cols > 16 ? (int)((cols + kW - 1) / kW) : 0;
+    };
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int kend, tiles;
+        shape(b0 + lane, kend, tiles);
+        total[0] += tiles ? 0 : kend;
+        total[1] += (int64_t)tiles * kend;
+    }
+    int chunk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        total[i] = __shfl(scan64(total[i], lane), 63, 64);
+        chunk[i] = range_keys(total[i], i ? p.pitems : p.titems, i ? p.pmin : p.tmin);
+    }
+    int64_t base[4] = {0, 0, 0, 0};
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int kend, tiles, at[4];
+        shape(b0 + lane, kend, tiles);
+        const int64_t nt = tiles ? 0 : (kend + chunk[0] - 1) / chunk[0];
+        const int64_t np = tiles ? (kend + chunk[1] - 1) / chunk[1] : 0;
+        const int64_t x[4] = {nt, parts_of(nt, 1), np * tiles, parts_of(np, tiles)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t incl = scan64(x[i], lane);
+            at[i] = (int)min(base[i] + incl - x[i], (int64_t)1 << 30);
+            base[i] += __shfl(incl, 63, 64);
+        }
+        if (b0 + lane < p.B) p.plan[b0 + lane] = make_int4(at[0], at[1], at[2], at[3]);
+    }
+    if (lane == 0)
+        p.plan[p.B] = make_int4((int)min(base[0], (int64_t)1 << 30), chunk[0],
+                                (int)min(base[2], (int64_t)1 << 30), chunk[1]);
+}
+
+// Pages: unit `i` (over KV) and kv head h of the token or prompt tiles; false: none.
+template <bool F32, bool PROMPT>
+__device__ __forceinline__ bool page_unit(const Params& p, int i, int h, Unit& un, Seq& s) {
+    constexpr int kW = PROMPT ? prompt_width(F32 ? ORTMI_F32 : ORTMI_F16) : 16;
+    const int lane = threadIdx.x & 63;
+    const int4 all = p.plan[p.B];
+    if (i >= (PROMPT ? all.z : all.x)) return false;
+    // The last sequence with at most i units in front, 64 places at a time.
+    int lo = 0, len = p.B;
+    while (len > 1) {
+        const int step = (len + 63) / 64, at = lane * step;
+        const int4 e = p.plan[lo + min(at, len - 1)];
+        const uint64_t le = __ballot(at < len && (PROMPT ? e.z : e.x) <= i);
+        const int skip = max(__popcll(le) - 1, 0) * step;
+        lo = uniform(lo + skip);
+        len = uniform(min(step, len - skip));
+    }
+    const int4 e = p.plan[lo];
+    s = sequence<true>(p, lo);
+    const int G = p.H / p.KV, chunk = PROMPT ? all.w : all.y, j = i - (PROMPT ? e.z : e.x);
+    int first = PROMPT ? e.w : e.y, tile = 0;
+    un.split = j;
+    if constexpr (PROMPT) {
+        const int n = (s.keys_to(s.rows - 1, p.limit) + chunk - 1) / chunk;
+        tile = j / n;
+        un.split = j - tile * n;
+        first += tile * n;
+    }
+    un.b = lo;
+    un.h = h;
+    un.c0 = tile * kW;
+    const int kend = s.keys_to((min(un.c0 + kW, s.rows * G) - 1) / G, p.limit);
+    un.n = (kend + chunk - 1) / chunk;
+    un.k0 = un.split * chunk;
+    un.k1 = min(un.k0 + chunk, kend);
+    un.first = (int64_t)first * p.KV + h;
+    un.step = p.KV;
+    un.part = PROMPT ? p.ppart : p.part;
+    un.ml = PROMPT ? p.pml : p.ml;
+    return un.split < un.n;
+}
+
+// Slabs: unit `i` of the tile and its sequence, also of tiles whose rows are all padding (k0 =
+// k1 = 0, one range).
+template <bool F32, bool PROMPT>
+__device__ __forceinline__ bool slab_unit(const Params& p, int i, Unit& un, Seq& s) {
+    constexpr int kW = PROMPT ? prompt_width(F32 ? ORTMI_F32 : ORTMI_F16) : 16;
+    const int G = p.H / p.KV;
+    int chunk = p.chunk, tile = 0;
+    un.part = p.part;
+    un.ml = p.ml;
+    if (PROMPT || !p.planned) {
+        // (range, tile, slab), the slab running fastest (slabs of one residue modulo 8 stay on
+        // one XCD). Later tiles, which see more keys, come first.
+        const int slabs = p.B * p.KV, rem = i % (slabs * p.ntile), slab = rem % slabs;
+        tile = p.ntile - 1 - rem / slabs;
+        un.b = slab / p.KV;
+        un.h = slab % p.KV;
+        un.split = i / (slabs * p.ntile);
+        un.first = ((int64_t)slab * p.ntile + tile) * p.nsplit;
+        un.step = 1;
+    } else {
+        // At most 64 sequences, a lane each: ranges of equal size (plan_units()).
+        const int lane = threadIdx.x & 63, item = i / p.KV;
+        const int kend = lane < p.B ? sequence<false>(p, lane).keys_to(p.S - 1, p.limit) : 0;
+        int64_t total = kend;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
+        chunk = uniform(range_keys(total, p.titems, p.tmin));
+        const int n = lane < p.B ? max(1, (kend + chunk - 1) / chunk) : 0;
+        int at = n, part = n > 1 ? n : 0;
+        const int own = part;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(at, o, 64), v = __shfl_up(part, o, 64);
+            at += lane >= o ? u : 0;
+            part += lane >= o ? v : 0;
+        }
+        const int b = uniform(__popcll(__ballot(at <= item)));  // sequences that end before it
+        if (b >= p.B) return false;
+        un.b = b;
+        un.h = i % p.KV;
+        un.split = item - uniform(__shfl(at - n, b, 64));
+        un.first = (int64_t)uniform(__shfl(part - own, b, 64)) * p.KV + un.h;
+        un.step = p.KV;
+    }
+    s = sequence<false>(p, un.b);
+    un.c0 = tile * kW;
+    un.k0 = un.k1 = 0;
+    un.n = 1;
+    if (un.c0 / G >= s.real) return un.split == 0;
+    const int kend = s.keys_to((min(un.c0 + kW, s.rows * G) - 1) / G, p.limit);
+    un.n = (kend + chunk - 1) / chunk;
+    un.k0 = un.split * chunk;
+    un.k1 = min(un.k0 + chunk, kend);
+    return un.split < un.n;
+}
+
+// New keys and values into the cache: a group of lanes per (token, kv head, key or value). Pages: the
+// first workgroup plans the units.
 template <int CODE, int HD, bool F32, bool PAGED>  // HD 0: any
 __global__ __launch_bounds__(256) void append_kernel(Params p) {
-    int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    constexpr int W = kRowLanes<HD>;
+    int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / W;
     if constexpr (PAGED) {
         if (blockIdx.x == 0) {
-            if (threadIdx.x < 64 && p.tiles) list_tiles(p);
+            if (threadIdx.x < 64 && p.plan) {
+                if (p.dtype == ORTMI_F32) plan_units<true>(p);
+                else plan_units<false>(p);
+            }
             return;
         }
-        item -= 16;
+        item -= 256 / W;
     }
     const int per = 2 * p.KV;
     const int64_t tok = item / per;
@@ -1034,9 +1250,9 @@ __global__ __launch_bounds__(256) void append_kernel(Params p) {
     const int r = (int)tok - s.tok0;
     if (r >= s.real) return;
     if constexpr (HD > 0)
-        append_piece<CODE, HD, F32, PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV, threadIdx.x & 15);
+        append_piece<CODE, HD, F32, PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV, threadIdx.x % W);
     else
-        append_row<PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV, threadIdx.x & 15);
+        append_row<PAGED>(p, b, s, r, hv % p.KV, hv >= p.KV, threadIdx.x % W);
 }
 
 // A tile that attends nothing: padded rows.
@@ -1052,69 +1268,38 @@ __device__ __forceinline__ void zero_rows(const Params& p, const Seq& s, int h, 
     }
 }
 
-// Slabs. Workgroups: (range, tile, slab), the slab running fastest (slabs of one residue
-// modulo 8 then stay on one XCD). Later tiles, which see more keys, come first. Where a
-// sequence's columns are one tile, the workgroup whose range holds the new rows writes them to
-// the cache itself.
+// Slabs, a workgroup for each unit. Where a sequence's columns are one tile, the workgroup whose
+// range holds the new rows writes them to the cache itself.
 template <int CODE, int HD, bool F32, bool PROMPT>
 __global__ __launch_bounds__(PROMPT ? 512 : 256, 2) void tile_kernel(Params p) {
     using SH = std::conditional_t<PROMPT, PromptShared<CODE, HD, F32>, TokenShared<HD, F32>>;
     __shared__ SH sh;
-    constexpr int kCols = PROMPT ? prompt_width(F32 ? ORTMI_F32 : ORTMI_F16) : 16;
-    const int slabs = p.B * p.KV;
-    const int split = blockIdx.x / (slabs * p.ntile), rem = blockIdx.x % (slabs * p.ntile);
-    const int tile = p.ntile - 1 - rem / slabs, slab = rem % slabs, b = slab / p.KV, h = slab % p.KV;
-    const Seq s = sequence<false>(p, b);
-    const int G = p.H / p.KV, c0 = tile * kCols;
-    if (c0 / G >= s.real) {
-        if (split == 0) zero_rows<HD, F32>(p, s, h, c0, kCols);
+    Unit un;
+    Seq s;
+    if (!slab_unit<F32, PROMPT>(p, blockIdx.x, un, s)) return;
+    if (un.k0 == un.k1) {
+        zero_rows<HD, F32>(p, s, un.h, un.c0, PROMPT ? prompt_width(F32 ? ORTMI_F32 : ORTMI_F16) : 16);
         return;
     }
-    const int kend = s.keys_to((min(c0 + kCols, s.rows * G) - 1) / G, p.limit);
-    const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, kend);
-    if (k0 >= kend) return;
     if (p.fused) {
-        append_rows<CODE, HD, F32, false>(p, b, s, max(k0 - s.past, 0), min(k1 - s.past, s.real), h);
+        append_rows<CODE, HD, F32, false>(p, un.b, s, max(un.k0 - s.past, 0),
+                                          min(un.k1 - s.past, s.real), un.h);
         __syncthreads();
     }
-    const int nsplit = (kend + p.chunk - 1) / p.chunk;
-    if constexpr (PROMPT)
-        prompt_tile<CODE, HD, F32, false>(p, s, b, h, c0, k0, k1, split, nsplit, sh);
-    else
-        token_tile<CODE, HD, F32, false>(p, s, b, h, k0, k1, split, nsplit, sh);
+    if constexpr (PROMPT) prompt_tile<CODE, HD, F32, false>(p, s, un, sh);
+    else token_tile<CODE, HD, F32, false>(p, s, un, sh);
 }
 
-// Pages, sequences of at most 16 columns: workgroups (range, sequence, kv head).
-template <int CODE, int HD, bool F32>
-__global__ __launch_bounds__(256, 2) void page_token_kernel(Params p) {
-    __shared__ TokenShared<HD, F32> sh;
-    const int slabs = p.B * p.KV, split = blockIdx.x / slabs, slab = blockIdx.x % slabs;
-    const int b = slab / p.KV, h = slab % p.KV, G = p.H / p.KV;
-    const Seq s = sequence<true>(p, b);
-    if (s.rows == 0 || s.rows * G > 16) return;
-    const int kend = s.keys_to(s.rows - 1, p.limit);
-    const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, kend);
-    if (k0 >= kend) return;
-    token_tile<CODE, HD, F32, true>(p, s, b, h, k0, k1, split, (kend + p.chunk - 1) / p.chunk, sh);
-}
-
-// Pages, the other sequences: a workgroup for each (range, listed tile, kv head), those past
-// the list's end with nothing to do.
-template <int CODE, int HD, bool F32>
-__global__ __launch_bounds__(512, 2) void page_tile_kernel(Params p) {
-    constexpr int kCols = prompt_width(F32 ? ORTMI_F32 : ORTMI_F16);
-    __shared__ PromptShared<CODE, HD, F32> sh;
-    const int G = p.H / p.KV, per = p.max_tiles * p.KV;
-    const int split = blockIdx.x / per, rem = blockIdx.x % per, h = rem % p.KV, i = rem / p.KV;
-    if (i >= *p.tile_count) return;
-    const int2 tl = p.tiles[i];
-    const int b = tl.x, c0 = tl.y;
-    const Seq s = sequence<true>(p, b);
-    const int kend = s.keys_to((min(c0 + kCols, s.rows * G) - 1) / G, p.limit);
-    const int k0 = split * p.tile_chunk, k1 = min(k0 + p.tile_chunk, kend);
-    if (k0 >= kend) return;
-    prompt_tile<CODE, HD, F32, true>(p, s, b, h, c0, k0, k1, split,
-                                     (kend + p.tile_chunk - 1) / p.tile_chunk, sh);
+// Pages, the same, of sequences with at most 16 columns (token tiles) and with more.
+template <int CODE, int HD, bool F32, bool PROMPT>
+__global__ __launch_bounds__(PROMPT ? 512 : 256, 2) void page_kernel(Params p) {
+    using SH = std::conditional_t<PROMPT, PromptShared<CODE, HD, F32>, TokenShared<HD, F32>>;
+    __shared__ SH sh;
+    Unit un;
+    Seq s;
+    if (!page_unit<F32, PROMPT>(p, blockIdx.x / p.KV, blockIdx.x % p.KV, un, s)) return;
+    if constexpr (PROMPT) prompt_tile<CODE, HD, F32, true>(p, s, un, sh);
+    else token_tile<CODE, HD, F32, true>(p, s, un, sh);
 }
 
 // New rows and attention for one code; in kvq_int8.hip, kvq_int4.hip and kvq_fp8.hip.
@@ -1122,31 +1307,37 @@ int tiles_int8(const Params& p, bool paged, hipStream_t st);
 int tiles_int4(const Params& p, bool paged, hipStream_t st);
 int tiles_fp8(const Params& p, bool paged, hipStream_t st);
 
+inline int64_t slab_units(const Params& p) {
+    return p.planned ? (int64_t)p.tgrid * p.KV : (int64_t)p.B * p.KV * p.ntile * p.nsplit;
+}
+
 template <int CODE, int HD, bool F32>
 int launch_tiles(const Params& p, bool paged, hipStream_t st) {
     const int G = p.H / p.KV;
-    const dim3 rows((unsigned)(((int64_t)p.T * 2 * p.KV + 15) / 16 + (paged ? 1 : 0)));
+    constexpr int kItems = 256 / kRowLanes<HD>;
+    const dim3 rows((unsigned)(((int64_t)p.T * 2 * p.KV + kItems - 1) / kItems + (paged ? 1 : 0)));
     if (p.pieces && !p.fused) {
         if (paged) hipLaunchKernelGGL((append_kernel<CODE, HD, F32, true>), rows, dim3(256), 0, st, p);
         else hipLaunchKernelGGL((append_kernel<CODE, HD, F32, false>), rows, dim3(256), 0, st, p);
         if (int rc = check_launch("kv append")) return rc;
     }
     if (!paged) {
-        const dim3 grid((unsigned)(p.B * p.KV * p.ntile * p.nsplit));
         if (p.S * G <= 16)
-            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, false>), grid, dim3(256), 0, st, p);
+            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, false>), dim3((unsigned)slab_units(p)),
+                               dim3(256), 0, st, p);
         else
-            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, true>), grid, dim3(512), 0, st, p);
+            hipLaunchKernelGGL((tile_kernel<CODE, HD, F32, true>), dim3((unsigned)slab_units(p)),
+                               dim3(512), 0, st, p);
         return check_launch("kv tiles");
     }
-    if (G <= 16) {
-        hipLaunchKernelGGL((page_token_kernel<CODE, HD, F32>),
-                           dim3((unsigned)(p.B * p.KV * p.nsplit)), dim3(256), 0, st, p);
+    if (p.tgrid) {
+        hipLaunchKernelGGL((page_kernel<CODE, HD, F32, false>), dim3((unsigned)((int64_t)p.tgrid * p.KV)),
+                           dim3(256), 0, st, p);
         if (int rc = check_launch("kv page tokens")) return rc;
     }
-    if ((int64_t)p.T * G <= 16) return ORTMI_OK;  // no sequence has more than 16 columns
-    hipLaunchKernelGGL((page_tile_kernel<CODE, HD, F32>),
-                       dim3((unsigned)(p.max_tiles * p.KV * p.tile_nsplit)), dim3(512), 0, st, p);
+    if (!p.pgrid) return ORTMI_OK;
+    hipLaunchKernelGGL((page_kernel<CODE, HD, F32, true>), dim3((unsigned)((int64_t)p.pgrid * p.KV)),
+                       dim3(512), 0, st, p);
     return check_launch("kv page tiles");
 }
 
