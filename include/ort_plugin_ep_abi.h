@@ -89,6 +89,7 @@ typedef enum ONNXTensorElementDataType {
     ONNX_TENSOR_ELEMENT_DATA_TYPE_COMPLEX64 = 14,
     ONNX_TENSOR_ELEMENT_DATA_TYPE_COMPLEX128 = 15,
     ONNX_TENSOR_ELEMENT_DATA_TYPE_BFLOAT16 = 16,
+    ONNX_TENSOR_ELEMENT_DATA_TYPE_FLOAT8E4M3FN = 17,
 } ONNXTensorElementDataType;
 
 typedef enum ONNXType {

@@ -32,6 +32,7 @@ size_t dtype_size(int dt) {
         case ONNX_TENSOR_ELEMENT_DATA_TYPE_DOUBLE: return 8;
         case ONNX_TENSOR_ELEMENT_DATA_TYPE_UINT8:
         case ONNX_TENSOR_ELEMENT_DATA_TYPE_INT8:
+        case ONNX_TENSOR_ELEMENT_DATA_TYPE_FLOAT8E4M3FN:
         case ONNX_TENSOR_ELEMENT_DATA_TYPE_BOOL: return 1;
         default: return 0;
     }
@@ -282,6 +283,44 @@ std::string claim_matmulnbits(const NodeDesc& n, const GraphIR& g) {
 }
 
 // rust/src/ops/attention.rs:1527-1738, restricted to what the gfx950 kernels run.
+// A GroupQueryAttention whose cache holds codes (int8, fp8 e4m3, or int4 two a uint8) with
+// static fp32 scales, inputs 12 and 13: one, or one for each kv head and channel.
+std::string claim_quantized_kv(const NodeDesc& n, const GraphIR& g, int64_t KV, int64_t hd) {
+    const char* types[2] = {"k_quant_type", "v_quant_type"};
+    for (int i = 0; i < 2; ++i) {
+        const std::string t = n.attr_str(types[i], "NONE");
+        REQUIRE(t == "PER_TENSOR" || t == "PER_CHANNEL",
+                "a quantized KV cache needs k_quant_type and v_quant_type PER_TENSOR or PER_CHANNEL");
+        REQUIRE(n.has_input(12 + i) && n.has_input(3 + i),
+                "a quantized KV cache needs past key/value and their scales");
+        auto* sc = val(g, n, 12 + i);
+        int64_t count = 1;
+        REQUIRE(sc && sc->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_FLOAT && sc->has_shape,
+                "quantized KV cache scales must be fp32 of known shape");
+        for (int64_t d : sc->dims) count *= d;
+        REQUIRE(count == (t == "PER_TENSOR" ? 1 : KV * hd),
+                "quantized KV cache scales must be one, or [kv_num_heads, head_size]");
+        auto* past = val(g, n, 3 + i);
+        REQUIRE(past && past->has_shape && past->dims.size() == 4, "past key/value must be rank 4");
+        const bool nibbles = past->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_UINT8;
+        REQUIRE(nibbles || past->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_INT8 ||
+                    past->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_FLOAT8E4M3FN,
+                "a quantized KV cache must be int8, uint8 (int4) or fp8 e4m3");
+        REQUIRE(past->dtype == val(g, n, 3)->dtype, "both caches must have one type");
+        REQUIRE(past->dims[1] == KV && past->dims[3] == (nibbles ? hd / 2 : hd),
+                "quantized past must be [batch, kv_num_heads, capacity, head_size]");
+        const int64_t bits = n.attr_int("kv_cache_bit_width", 0);
+        REQUIRE(bits == 0 || bits == (nibbles ? 4 : 8),
+                "kv_cache_bit_width does not match the cache's type");
+    }
+    REQUIRE(!n.has_input(10), "attention_bias with a quantized KV cache is not supported");
+    REQUIRE(n.attr_int("sliding_window_cache", 0) == 0 && n.attr_int("local_window_size", -1) == -1,
+            "a window with a quantized KV cache is not supported");
+    REQUIRE(n.outputs.size() >= 3 && !n.outputs[1].empty() && !n.outputs[2].empty(),
+            "a quantized KV cache needs present key/value");
+    return "";
+}
+
 std::string claim_gqa(const NodeDesc& n, const GraphIR& g) {
     REQUIRE(n.inputs.size() >= 7 && n.inputs.size() <= 16, "GroupQueryAttention needs 7-16 inputs");
     REQUIRE(!n.outputs.empty() && !n.outputs[0].empty(), "GroupQueryAttention needs an output");
@@ -314,7 +353,13 @@ std::string claim_gqa(const NodeDesc& n, const GraphIR& g) {
     REQUIRE(seq && seq->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_INT32, "seqlens_k must be int32");
     REQUIRE(tot && tot->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_INT32,
             "total_sequence_length must be int32");
-    if (n.has_input(3)) {
+    const bool quantized = n.has_input(12) || n.has_input(13) ||
+                           n.attr_str("k_quant_type", "NONE") != "NONE" ||
+                           n.attr_str("v_quant_type", "NONE") != "NONE";
+    if (quantized) {
+        const std::string why = claim_quantized_kv(n, g, KV, qhd);
+        if (!why.empty()) return why;
+    } else if (n.has_input(3)) {
         auto* pk = val(g, n, 3);
         REQUIRE(pk && pk->has_shape && pk->dims.size() == 4, "past_key must be rank 4");
         REQUIRE(pk->dims[3] == qhd && pk->dims[1] == KV,
@@ -325,7 +370,8 @@ std::string claim_gqa(const NodeDesc& n, const GraphIR& g) {
     const bool rotary = n.attr_int("do_rotary", 0) != 0;
     REQUIRE(!rotary || (n.has_input(7) && n.has_input(8)), "do_rotary needs cos/sin caches");
     // Every float input shares the output dtype (attention.rs:1583-1615).
-    std::vector<size_t> floats = {0, 1, 2, 3, 4};
+    std::vector<size_t> floats = {0, 1, 2};
+    if (!quantized) floats.insert(floats.end(), {3, 4});
     if (rotary) floats.insert(floats.end(), {7, 8});
     floats.insert(floats.end(), {10, 14, 15});
     for (size_t i : floats) {
@@ -343,10 +389,6 @@ std::string claim_gqa(const NodeDesc& n, const GraphIR& g) {
                 "attention_bias heads must be 1 or num_heads");
     }
     REQUIRE(!n.has_input(11), "head_sink is not supported");
-    REQUIRE(!n.has_input(12) && !n.has_input(13), "quantized KV cache scales are not supported");
-    REQUIRE(n.attr_str("k_quant_type", "NONE") == "NONE" &&
-                n.attr_str("v_quant_type", "NONE") == "NONE",
-            "quantized KV cache is not supported");
     REQUIRE(n.has_input(14) == n.has_input(15),
             "q_norm_weight and k_norm_weight must be provided together");
     for (size_t i : {14, 15})

@@ -1002,6 +1002,56 @@ void Plan::run_node(const NodeDesc& n, const OrtApi* a, OrtKernelContext* ctx) {
         const bool packed = kp == nullptr;
         const int64_t hd = packed ? q.dims[2] / (H + 2 * KV) : q.dims[2] / H;
         const int64_t cap = pk ? pk->dims[2] : 0;
+        if (n.has_input(12)) {  // codes with scales; claim_quantized_kv: past and present given
+            if (capturing_) fail("GroupQueryAttention form is not capturable");
+            capturable_ = false;
+            if (!pk || !pv || pk->dims.size() != 4 || pv->dims != pk->dims || pk->dims[0] != B)
+                fail("GroupQueryAttention: quantized past key/value must have one shape",
+                     ORT_INVALID_ARGUMENT);
+            Tensor& seq = need(5);
+            if (seq.numel() != B)
+                fail("GroupQueryAttention: seqlens_k must have one value per batch",
+                     ORT_INVALID_ARGUMENT);
+            for (Tensor* t : {pk, pv})
+                if (t->lazy) {
+                    check_hip(hipMemcpyAsync(t->ptr, t->host, (size_t)t->numel() * dtype_size(t->dtype),
+                                             hipMemcpyHostToDevice, stream_),
+                              "stage past");
+                    t->lazy = false;
+                }
+            const bool rotary = n.attr_int("do_rotary", 0) != 0;
+            Tensor* cs = rotary ? in(7) : nullptr;
+            Tensor* sn = rotary ? in(8) : nullptr;
+            Tensor* qnw = in(14);
+            Tensor* knw = in(15);
+            const int32_t code = pk->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_INT8    ? ORTMI_INT8
+                                 : pk->dtype == ONNX_TENSOR_ELEMENT_DATA_TYPE_UINT8 ? ORTMI_INT4
+                                                                                    : ORTMI_F8E4M3;
+            const int64_t fits = (int64_t)total - S;  // tokens before this call's, or the cache grows
+            std::vector<int64_t> pdims = pk->dims;
+            if (fits < 0 || fits >= cap) pdims[2] = cap + S;
+            const int cache_type = pk->dtype;
+            void* optr = out_tensor(outname(0), q.dtype, {B, S, H * hd}, a, ctx).ptr;
+            void* prk = out_tensor(outname(1), cache_type, pdims, a, ctx).ptr;
+            void* prv = out_tensor(outname(2), cache_type, pdims, a, ctx).ptr;
+            const size_t wsb = ortmi_group_query_attention_quantized_workspace_size(
+                B, S, H, KV, hd, pdims[2]);
+            void* ws = workspace(wsb);
+            check_kernel(ortmi_group_query_attention_quantized(
+                             q.ptr, kp ? kp->ptr : nullptr, vp ? vp->ptr : nullptr, pk->ptr,
+                             pv->ptr, cap, total, static_cast<const int32_t*>(seq.ptr),
+                             cs ? cs->ptr : nullptr, sn ? sn->ptr : nullptr, cs ? cs->dims[1] : 0,
+                             cs ? cs->dims[0] : 0, qnw ? qnw->ptr : nullptr,
+                             knw ? knw->ptr : nullptr, n.attr_float("qk_norm_epsilon", 1e-6f),
+                             static_cast<const float*>(need(12).ptr),
+                             static_cast<const float*>(need(13).ptr),
+                             n.attr_str("k_quant_type", "NONE") == "PER_CHANNEL",
+                             n.attr_str("v_quant_type", "NONE") == "PER_CHANNEL", code, optr, prk,
+                             prv, B, S, H, KV, hd, n.attr_float("scale", 0.f),
+                             (int32_t)n.attr_int("rotary_interleaved", 0), kdt(q.dtype), ws, wsb, st),
+                         "GroupQueryAttention");
+            return;
+        }
         int64_t vpast = total - S;
         bool shared;
         if (vpast < 0 || vpast > cap) {
