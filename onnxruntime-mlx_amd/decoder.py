@@ -11,8 +11,8 @@ symmetric, with fp16 scales |N(0, 0.02)|.
 The KV cache is device resident with a fixed capacity: each layer's present
 output is bound to its past input buffer, so GroupQueryAttention writes the new
 rows in place (the shared-buffer contract, rust/src/ops/attention.rs:893-902).
-Greedy decoding takes the argmax on the device and feeds it back as the next
-input id, so a decode step reads nothing back to the host but total_sequence_length.
+The next token, the argmax or a sampled one, is taken on the device and fed back as
+the next input id, so a decode step reads nothing back to the host but total_sequence_length.
 """
 
 from __future__ import annotations
@@ -24,7 +24,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from . import check, load_kernels
+from . import check, load_kernels, ops
 from . import harness as hx
 
 
@@ -209,7 +209,7 @@ def build_graph(cfg: DecoderConfig, w, cap: int, layer_metadata: bool = False,
 
 
 class DecoderRunner:
-    """Greedy generation through the EP with a device-resident KV cache.
+    """Generation through the EP with a device-resident KV cache: greedy, or sampled.
 
     seqlens_k and total_sequence_length are host inputs (pinned), as ONNX Runtime
     keeps them; logits and KV are bound to device buffers (IOBinding).
@@ -225,14 +225,27 @@ class DecoderRunner:
     argmax_node the ArgMax output is bound to host memory, where a serving loop
     reads the token. Otherwise the ids stay in HBM and the argmax output is fed
     back in place.
+
+    sampling: draw each token from the last logits row with sample_rows instead of taking
+    the largest: its temperature, top_k, top_p and min_p, and seed (0) of the uniform
+    numbers, which reset() starts again. Not with argmax_node.
     """
 
     def __init__(self, cfg: DecoderConfig, weights, cap: int, max_prompt: int,
                  layer_metadata: bool = False, argmax_node: bool = False,
-                 host_feeds: bool = False, norm_stats: bool = False):
+                 host_feeds: bool = False, norm_stats: bool = False, sampling: dict = None):
         import torch
 
+        if sampling is not None and argmax_node:
+            raise ValueError("sampling needs logits: not with argmax_node")
         self.torch = torch
+        self.sampling = None if sampling is None else dict(sampling)
+        if self.sampling is not None:
+            self.seed = int(self.sampling.pop("seed", 0))
+            if bad := set(self.sampling) - {"temperature", "top_k", "top_p", "min_p"}:
+                raise ValueError(f"unknown sampling settings: {sorted(bad)}")
+            self.uniform = torch.empty(1, dtype=torch.float32, device="cuda")
+            self.random = torch.Generator(device="cuda").manual_seed(self.seed)
         self.cfg = cfg
         self.cap = cap
         self.argmax_node = argmax_node
@@ -282,6 +295,8 @@ class DecoderRunner:
 
     def reset(self):
         self.length = 0
+        if self.sampling is not None:
+            self.random.manual_seed(self.seed)
 
     def run(self, ids, S: int):
         """Forward S new tokens (device int64 [1, S]); logits land in self.logits[:, :S]."""
@@ -300,9 +315,15 @@ class DecoderRunner:
             self.next_id = self._first[self._flip] if S == 1 else out[:, S - 1:S]
             self._flip ^= 1
 
-    def argmax_last(self, S: int):
+    def next_token(self, S: int):
+        """The next input id from the logits of the run's last row."""
         if self.argmax_node:
             return  # the graph's ArgMax already wrote next_id
+        if self.sampling is not None:
+            self.uniform.uniform_(generator=self.random)
+            ids, _ = ops.sample_rows(self.logits[0, S - 1:S], self.uniform, **self.sampling)
+            self.next_id.copy_(ids.view(1, 1))
+            return
         st = ctypes.c_void_p(self.torch.cuda.current_stream().cuda_stream)
         last = self.logits[0, S - 1]
         check(self.lib.ortmi_argmax_rows(ctypes.c_void_p(last.data_ptr()),
@@ -320,7 +341,7 @@ class DecoderRunner:
         else:
             self.ids[0, :S].copy_(ids)
             self.run(self.ids[:, :S], S)
-        self.argmax_last(S)
+        self.next_token(S)
 
     def decode_step(self):
         if self.host_feeds:
@@ -330,10 +351,10 @@ class DecoderRunner:
             self.run(self.ids_host[:, :1], 1)
         else:
             self.run(self.next_id, 1)
-        self.argmax_last(1)
+        self.next_token(1)
 
     def generate(self, prompt: np.ndarray, steps: int):
-        """Greedy: returns (tokens, prefill seconds, per-decode-step seconds)."""
+        """Returns (tokens, prefill seconds, per-decode-step seconds)."""
         torch = self.torch
         self.reset()
         torch.cuda.synchronize()
