@@ -318,27 +318,27 @@ def _operand(what, name, t, dtype, device):
     """Device address of an operand of the given dtype (None: absent)."""
     if t is None:
         return None
+    if t.dtype is dtype and t.device == device and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype != dtype:
         raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{what}: {name} must be on {device}, as the query is")
-    if not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{what}: {name} must be contiguous")
 
 
 def _kv_scales(what, k_scale, v_scale, k_quant_type, v_quant_type, KV, hd, device):
     """(k address, v address, k per channel, v per channel)."""
-    out = []
-    for name, s, kind in (("k", k_scale, k_quant_type), ("v", v_scale, v_quant_type)):
-        if kind not in ("PER_TENSOR", "PER_CHANNEL"):
+    k_channel, v_channel = k_quant_type == "PER_CHANNEL", v_quant_type == "PER_CHANNEL"
+    for name, s, kind, channel in (("k", k_scale, k_quant_type, k_channel),
+                                   ("v", v_scale, v_quant_type, v_channel)):
+        if not channel and kind != "PER_TENSOR":
             raise ValueError(f"{what}: {name}_quant_type must be PER_TENSOR or PER_CHANNEL")
-        if s is None or s.numel() != (KV * hd if kind == "PER_CHANNEL" else 1):
+        if s is None or s.numel() != (KV * hd if channel else 1):
             raise ValueError(f"{what}: {name}_scale must hold one number, or with PER_CHANNEL "
                              "kv_num_heads * head_size")
-        out.append((_operand(what, name + "_scale", s, torch.float32, device),
-                    int(kind == "PER_CHANNEL")))
-    return out[0][0], out[1][0], out[0][1], out[1][1]
+    return (_operand(what, "k_scale", k_scale, torch.float32, device),
+            _operand(what, "v_scale", v_scale, torch.float32, device), k_channel, v_channel)
 
 
 def _rotary_operands(what, do_rotary, cos_cache, sin_cache, hd, dtype, device):
@@ -355,6 +355,8 @@ def _rotary_operands(what, do_rotary, cos_cache, sin_cache, hd, dtype, device):
 
 
 def _norm_operands(what, q_norm_weight, k_norm_weight, hd, dtype, device):
+    if q_norm_weight is None and k_norm_weight is None:
+        return None, None
     for w in (q_norm_weight, k_norm_weight):
         if w is not None and w.numel() != hd:
             raise ValueError(f"{what}: q/k norm weights must have head_size elements")
@@ -435,7 +437,9 @@ def group_query_attention_quantized(query, key, value, past_key, past_value, k_s
         present_key = torch.empty(shape, dtype=cdt, device=device)
     if present_value is None:
         present_value = torch.empty(shape, dtype=cdt, device=device)
-    if present_key.shape != shape or present_value.shape != shape:
+    own_key, own_value = present_key is not past_key, present_value is not past_value
+    if (own_key or shape != past_key.shape) and present_key.shape != shape or \
+            (own_value or shape != past_value.shape) and present_value.shape != shape:
         raise ValueError(f"{what}: present key/value have the wrong shape for the contract")
     if seqlens_k is not None and seqlens_k.numel() != B:
         raise ValueError(f"{what}: seqlens_k must have one value per sequence")
@@ -443,21 +447,22 @@ def group_query_attention_quantized(query, key, value, past_key, past_value, k_s
                                 hd, device)
     rotary = _rotary_operands(what, do_rotary, cos_cache, sin_cache, hd, dtype, device)
     norms = _norm_operands(what, q_norm_weight, k_norm_weight, hd, dtype, device)
-    out = torch.empty((B, S, num_heads * hd), dtype=dtype, device=device)
+    out = torch.empty_like(query) if key is not None and query.is_contiguous() else \
+        torch.empty((B, S, num_heads * hd), dtype=dtype, device=device)
     lib = load_kernels()
     need = lib.ortmi_group_query_attention_quantized_workspace_size(
         B, S, num_heads, kv_num_heads, hd, vp + S)
     ws, ws_bytes, _keep = _own_workspace(what, workspace, need, device)
+    pk = _operand(what, "past_key", past_key, cdt, device)
+    pv = _operand(what, "past_value", past_value, cdt, device)
     check(lib.ortmi_group_query_attention_quantized(
         _operand(what, "query", query, dtype, device), _operand(what, "key", key, dtype, device),
-        _operand(what, "value", value, dtype, device),
-        _operand(what, "past_key", past_key, cdt, device),
-        _operand(what, "past_value", past_value, cdt, device), cap, total,
+        _operand(what, "value", value, dtype, device), pk, pv, cap, total,
         _operand(what, "seqlens_k", seqlens_k, torch.int32, device), *rotary, *norms,
         qk_norm_epsilon, ks, vs, kc, vc, code, out.data_ptr(),
-        _operand(what, "present_key", present_key, cdt, device),
-        _operand(what, "present_value", present_value, cdt, device), B, S, num_heads,
-        kv_num_heads, hd, scale, rotary_interleaved, _dt(query), ws, ws_bytes, _stream(stream)))
+        _operand(what, "present_key", present_key, cdt, device) if own_key else pk,
+        _operand(what, "present_value", present_value, cdt, device) if own_value else pv, B, S,
+        num_heads, kv_num_heads, hd, scale, rotary_interleaved, _dt(query), ws, ws_bytes, _stream(stream)))
     return out, present_key, present_value
 
 

@@ -72,3 +72,52 @@ def test_refusals():
         dec.DecoderRunner(cfg, w, cap=64, max_prompt=16, argmax_node=True, sampling={})
     with pytest.raises(ValueError, match="top_n"):
         dec.DecoderRunner(cfg, w, cap=64, max_prompt=16, sampling=dict(top_n=3))
+
+
+def test_paged_cache_and_sampling_in_turn(ortmi):
+    """Tokens of two sequences: attention over quantised pages, logits, a drawn token, whose
+    query, key and value are the next step's. Every step against 64 bits."""
+    import torch
+    from kvq_ref import Attention, random_scales, rotary
+
+    H, KV, hd, blk, V, dt = 4, 2, 64, 16, 500, torch.float16
+    g = torch.Generator().manual_seed(8)
+    ks, vs = (random_scales(g, KV, hd, "int4", False) for _ in range(2))
+    cos, sin = rotary(g, 64, hd // 2, dt)
+    ref = Attention(dt, "int4", H, KV, hd, ks, vs, 0.0, cos, sin)
+    table = [torch.randn((V, n * hd), generator=g).to(dt) for n in (H, KV, KV)]
+    head = torch.randn((H * hd, V), generator=g) * 0.3
+    pages = [torch.zeros((8, blk, KV, hd // 2), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    bt = torch.tensor([[5, 2, 7], [1, 6, 0]], dtype=torch.int32).cuda()
+    kb = [torch.zeros((64, KV, hd // 2), dtype=torch.uint8) for _ in range(2)]
+    vb = [x.clone() for x in kb]
+    news, past = [list(range(20)), [3, 400, 17]], [0, 0]
+    for _ in range(8):
+        n = [len(x) for x in news]
+        q, k, v = (t[torch.tensor(news[0] + news[1])] for t in table)
+        out = ortmi.paged_attention_quantized(
+            q.cuda(), k.cuda(), v.cuda(), *pages, ks.cuda(), vs.cuda(),
+            torch.tensor([0, n[0], n[0] + n[1]], dtype=torch.int32).cuda(),
+            torch.tensor(past, dtype=torch.int32).cuda(), bt, cos.cuda(), sin.cuda(),
+            num_heads=H, kv_num_heads=KV, do_rotary=1)
+        torch.cuda.synchronize()
+        got, start = out.double().cpu(), 0
+        for b in range(2):
+            rows = slice(start, start + n[b])
+            pos = torch.arange(past[b], past[b] + n[b])
+            kb[b][pos], vb[b][pos] = ref.new_codes(k[rows], v[rows], pos)
+            end = past[b] + n[b]
+            o, tol = ref.rows(q[rows], pos, kb[b][:end], vb[b][:end],
+                              torch.ones(end, dtype=torch.bool))
+            assert ((got[rows] - o).abs() <= tol).all(), (b, past)
+            start += n[b]
+        last = torch.tensor([n[0] - 1, n[0] + n[1] - 1])
+        logits = (got[last].float() @ head).to(dt)
+        u = torch.rand(2, generator=g)
+        ids, _ = ortmi.sample_rows(logits.cuda(), u.cuda(), **SETTINGS)
+        for b in range(2):
+            cdf, want = drawn(logits[b].float().numpy(), float(u[b]), **SETTINGS)
+            assert np.abs(cdf - float(u[b])).min() > 1e-6
+            assert int(ids[b]) == want
+            past[b] += n[b]
+            news[b] = [want]
