@@ -49,7 +49,7 @@ struct Params {
     int ntile, nsplit, chunk;   // slabs: tiles of a sequence, ranges of `chunk` keys at most
     int planned;                // slabs, token tiles: ranges from the sequences' lengths
     float *ppart, *pml;         // pages: of prompt tiles
-    int pitems, pmin;           // prompt tiles: units over KV to come near, least keys of a range
+    int pparts, pmin;           // prompt tiles: units over KV in ppart, least keys of a range
     int4* plan;                 // pages: plan_units()
     int tgrid, pgrid;           // units over KV at most
     int fused;                  // slabs: the tiles write the new rows themselves

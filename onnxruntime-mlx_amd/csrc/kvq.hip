@@ -263,20 +263,21 @@ static size_t plan_pages(Params& p, char* ws) {
     const int64_t G = p.H / p.KV, cols = p.T * G, w = prompt_width(p.dtype);
     const int64_t seqs = std::min<int64_t>(p.B, p.T);
     p.titems = (int)std::max<int64_t>(1, kTokenUnits / p.KV);
-    p.pitems = (int)std::max<int64_t>(1, kPromptUnits / p.KV);
     p.tmin = kTokenLeast;
     p.pmin = kPromptLeast;
     p.tcols = (int)std::min<int64_t>(16, cols);
     p.tgrid = G > 16 ? 0 : (int)(p.titems + seqs);
     // Sequences with prompt tiles have 17 columns or more.
     const int64_t tiles = cols / w + std::min<int64_t>(seqs, cols / 17);
-    p.pgrid = tiles ? (int)(p.pitems + tiles) : 0;
+    p.pparts = (int)std::min<int64_t>(std::max<int64_t>(1, 2 * kPromptUnits / p.KV),
+                                      tiles * ((p.limit + (int64_t)p.pmin - 1) / p.pmin));
+    p.pgrid = tiles ? (int)(p.pparts + tiles) : 0;
     size_t at = align_up((size_t)(p.B + 1) * sizeof(int4));
     p.plan = reinterpret_cast<int4*>(ws);
     p.nsplit = p.limit > std::min(p.tmin, kPromptLeast) ? 2 : 1;
     if (p.nsplit == 1) return at;
     at = place_parts(p.part, p.ml, ws, at, std::min(p.tgrid, 2 * p.titems) * (int64_t)p.KV * p.tcols, p.hd);
-    return place_parts(p.ppart, p.pml, ws, at, std::min(p.pgrid, 2 * p.pitems) * p.KV * w, p.hd);
+    return place_parts(p.ppart, p.pml, ws, at, (int64_t)p.pparts * p.KV * w, p.hd);
 }
 
 // On the matrix cores where head size and alignment allow 16-byte loads and pages are whole

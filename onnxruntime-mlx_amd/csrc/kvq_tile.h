@@ -1072,6 +1072,9 @@ __device__ __forceinline__ int range_keys(int64_t total, int items, int least) {
     const int64_t per = (total / items + 128) & ~127LL;  // above total / items
     return (int)max((int64_t)least, min(per, (int64_t)kMostKeys));
 }
+// Keys of each of n ranges of equal size: n stays the least number of ranges of at most the
+// keys it was found with.
+__device__ __forceinline__ int even_keys(int keys, int n) { return ((keys + n - 1) / n + 127) & ~127; }
 // Units that n of a sequence's ranges put into part and ml: with one range, none.
 __device__ __forceinline__ int64_t parts_of(int64_t n, int64_t tiles) { return n > 1 ? n * tiles : 0; }
 
@@ -1084,17 +1087,48 @@ __device__ __forceinline__ int64_t scan64(int64_t x, int lane) {
     return x;
 }
 
+// Keys of a range of prompt tiles, for `seqs` sequences of which the longest has `most` keys;
+// shape(b, keys, tiles) gives each. A workgroup of prompt tiles has a CU of its own and kAround
+// keys' time around its loop, so that r rounds of ranges of c keys take about r (c + kAround): a
+// lane prices a number of ranges for the longest sequence. Workgroups start in order and wait for
+// the engine whose turn it is: short ranges between long ones do not fill gaps (four prompts of
+// 256 rows over 2200 to 5500 keys in ranges of 3584 and what remained: 160 us for 106 of work).
+template <typename F>
+__device__ __forceinline__ int prompt_keys(const Params& p, int seqs, int most, F shape) {
+    constexpr int kAround = 570, kCus = 256;
+    const int lane = threadIdx.x & 63;
+    int c = max(p.pmin, (most + 127) & ~127);
+    if (seqs > kCus) return c;  // enough of them
+    c = max(p.pmin, even_keys(most, lane + 1));
+    int64_t units = 0, parts = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int keys, tiles;
+        shape(b0 + lane, keys, tiles);
+        for (uint64_t left = __ballot(tiles > 0); left; left &= left - 1) {
+            const int j = __builtin_ctzll(left);
+            const int k = __shfl(keys, j, 64), t = __shfl(tiles, j, 64);
+            const int n = (k + c - 1) / c;
+            units += (int64_t)n * t;
+            parts += parts_of(n, t);
+        }
+    }
+    const int64_t rounds = (units * p.KV + kCus - 1) / kCus;
+    const float cost = parts <= p.pparts ? (float)rounds * (float)(c + kAround) : INFINITY;
+    const uint64_t best = __ballot(cost == -wave_max(-cost));  // (lane 0: no parts)
+    return __shfl(c, __builtin_ctzll(best), 64);
+}
+
 // Pages: the ranges, by one wave. Token tiles are those of sequences with at most 16 columns;
 // the others have prompt tiles, all over the ranges of the sequence's last. plan[b]: the units
 // (over KV) in front of sequence b, of token tiles x (in part: y), of prompt tiles z (in ppart:
-// w); plan[B]: all units x, z and the keys of a range y, w. Ranges of equal size, whatever the
-// sequences' lengths, keep the GPU evenly filled. Ranges that are not their tile's only one are
-// at most twice the units aimed at: n ranges of c keys, n > 1, lie over more than n c / 2 keys.
+// w); plan[B]: all units x, z and the most keys of a range y, w. Ranges of near equal size,
+// whatever the sequences' lengths, keep the GPU evenly filled. Of token tiles, units that are not
+// their tile's only one are at most twice those aimed at: n ranges for one of c keys, n > 1, lie
+// over more than n c / 2 keys.
 template <bool F32>
 __device__ __forceinline__ void plan_units(const Params& p) {
     constexpr int kW = prompt_width(F32 ? ORTMI_F32 : ORTMI_F16);
     const int lane = threadIdx.x & 63, G = p.H / p.KV;
-    int64_t total[2] = {0, 0};
     auto shape = [&](int b, int& kend, int& tiles) {
         kend = tiles = 0;
         if (b >= p.B) return;
@@ -1103,18 +1137,21 @@ __device__ __forceinline__ void plan_units(const Params& p) {
         if (s.rows > 0) kend = s.keys_to(s.rows - 1, p.limit);
         tiles = cols > 16 ? (int)((cols + kW - 1) / kW) : 0;
     };
+    int64_t total = 0;
+    int most = 0, seqs = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         int kend, tiles;
         shape(b0 + lane, kend, tiles);
-        total[0] += tiles ? 0 : kend;
-        total[1] += (int64_t)tiles * kend;
+        total += tiles ? 0 : kend;
+        most = max(most, tiles ? kend : 0);
+        seqs += __popcll(__ballot(tiles > 0));
     }
-    int chunk[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        total[i] = __shfl(scan64(total[i], lane), 63, 64);
-        chunk[i] = range_keys(total[i], i ? p.pitems : p.titems, i ? p.pmin : p.tmin);
+    for (int o = 32; o; o >>= 1) {
+        total += __shfl_xor(total, o, 64);
+        most = max(most, __shfl_xor(most, o, 64));
     }
+    const int chunk[2] = {range_keys(total, p.titems, p.tmin), seqs ? prompt_keys(p, seqs, most, shape) : 128};
     int64_t base[4] = {0, 0, 0, 0};
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         int kend, tiles, at[4];
@@ -1154,11 +1191,12 @@ __device__ __forceinline__ bool page_unit(const Params& p, int i, int h, Unit& u
     }
     const int4 e = p.plan[lo];
     s = sequence<true>(p, lo);
-    const int G = p.H / p.KV, chunk = PROMPT ? all.w : all.y, j = i - (PROMPT ? e.z : e.x);
+    const int G = p.H / p.KV, most = PROMPT ? all.w : all.y, j = i - (PROMPT ? e.z : e.x);
     int first = PROMPT ? e.w : e.y, tile = 0;
     un.split = j;
+    const int keys = s.keys_to(s.rows - 1, p.limit), n = (keys + most - 1) / most;
+    const int chunk = even_keys(keys, n);
     if constexpr (PROMPT) {
-        const int n = (s.keys_to(s.rows - 1, p.limit) + chunk - 1) / chunk;
         tile = j / n;
         un.split = j - tile * n;
         first += tile * n;
@@ -1217,6 +1255,7 @@ __device__ __forceinline__ bool slab_unit(const Params& p, int i, Unit& un, Seq&
         if (b >= p.B) return false;
         un.b = b;
         un.h = i % p.KV;
+        chunk = uniform(__shfl(even_keys(kend, max(n, 1)), b, 64));
         un.split = item - uniform(__shfl(at - n, b, 64));
         un.first = (int64_t)uniform(__shfl(part - own, b, 64)) * p.KV + un.h;
         un.step = p.KV;
