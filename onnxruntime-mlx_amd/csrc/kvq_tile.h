@@ -20,13 +20,18 @@
 // Token tiles: 16 columns. A workgroup's 4 waves take every fourth block of 32 keys of its
 // range and are joined at the end; keys and values go from memory into registers, where each
 // wave decodes its own. Memory binds it: 4 sequences of 131072 int8 keys, 8 heads of 128, 190
-// us, 5.65 TB/s.
+// us, 5.65 TB/s; 32 of 256 to 8192 in pages 64 us, 4.2 TB/s. A unit has about 8 us around its
+// loop (its place 2.5, rotated queries 2.3, the first loads, the join 1.3), which is all of a
+// short call: 512 keys, 12 us.
 //
 // Prompt tiles: 128 columns (fp32 64), 32 a wave, by two teams of 4 waves that take every other
 // block of 64 keys and are joined at the end. A team decodes its block together into LDS, a
 // quarter each, in the order that the products read: decoded once for 128 columns. Two buffers
 // a team, so that one barrier for two blocks suffices; the second team fills the waits of the
-// first, which the registers (200 of 256 at two waves a SIMD) leave no other wave for.
+// first, which the registers (220 of 256 at two waves a SIMD) leave no other wave for. One team
+// a workgroup and two workgroups a CU instead: a 2048-token prompt 76 us, not 71 (34.4 GFLOP,
+// 485 TFLOP/s; at 8160 keys before it 676). 128 keys take 2.1 to 2.7 us of a CU, issued vector
+// instructions beside matrix cores 24 % busy, and a unit has 12 us around its loop.
 #pragma once
 
 #include <algorithm>
