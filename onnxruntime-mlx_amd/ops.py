@@ -8,6 +8,7 @@ translator each follows is cited in its docstring.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -364,6 +365,18 @@ def _norm_operands(what, q_norm_weight, k_norm_weight, hd, dtype, device):
             _operand(what, "k_norm_weight", k_norm_weight, dtype, device))
 
 
+def _on_stream(call):
+    """With stream=, the call and what it allocates belong to that stream: memory that another
+    stream may still use, or will be given before the call has run, is not taken."""
+    @functools.wraps(call)
+    def on_stream(*args, stream=None, **kwargs):
+        if stream is None:
+            return call(*args, **kwargs)
+        with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
+            return call(*args, **kwargs)
+    return on_stream
+
+
 def _own_device(what, query):
     """The query's device, which has to be the current one (the stream's)."""
     if not query.is_cuda:
@@ -381,6 +394,7 @@ def _own_workspace(what, workspace, nbytes, device):
     return _operand(what, "workspace", workspace, torch.uint8, device), workspace.numel(), workspace
 
 
+@_on_stream
 def group_query_attention_quantized(query, key, value, past_key, past_value, k_scale, v_scale,
                                     seqlens_k, total_sequence_length, cos_cache=None,
                                     sin_cache=None, *, num_heads, kv_num_heads,
@@ -466,6 +480,7 @@ def group_query_attention_quantized(query, key, value, past_key, past_value, k_s
     return out, present_key, present_value
 
 
+@_on_stream
 def paged_attention_quantized(query, key, value, key_cache, value_cache, k_scale, v_scale,
                               cumulative_sequence_length, past_seqlens, block_table,
                               cos_cache=None, sin_cache=None, head_sink=None, q_norm_weight=None,
@@ -593,6 +608,7 @@ def skip_simplified_layer_norm(x, skip, gamma, bias=None, *, epsilon=1e-6, strea
 
 
 # -------------------------------------------------------------------- Sampling
+@_on_stream
 def sample_rows(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
                 workspace=None, stream=None):
     """One token per row of logits [..., V] (V up to 262144), drawn with one given uniform

@@ -110,3 +110,28 @@ def test_same_result_every_time(ortmi):
     for _ in range(5):
         assert torch.equal(ortmi.paged_attention_quantized(**args), first)
     check_paged(first, args, t)
+
+
+def test_the_stream_of_the_call(ortmi):
+    """stream=: run there, in order with its other work, whatever the current stream does."""
+    side = torch.cuda.Stream()
+    args, t = make_gqa(S=1, past=3000, hd=128)
+    pages, pt = make_paged(past=(2500, 700), new=(1, 30), hd=128)
+    logits = torch.randn((3, 5000), device="cuda")
+    u = torch.rand(3, device="cuda")
+    ids = ortmi.sample_rows(logits, u, top_k=40)[0]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # the calls wait behind this
+        fill = [args["query"].clone(), pages["query"].clone(), logits.clone()]
+    args["query"], pages["query"] = fill[:2]
+    out = ortmi.group_query_attention_quantized(**args, stream=side.cuda_stream)
+    paged = ortmi.paged_attention_quantized(**pages, stream=side.cuda_stream)
+    drawn = ortmi.sample_rows(fill[2], u, top_k=40, stream=side.cuda_stream)[0]
+    junk = [torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    side.synchronize()
+    torch.cuda.synchronize()
+    check_gqa(ortmi, out, t)
+    check_paged(paged, pages, pt)
+    assert torch.equal(drawn, ids)
+    del junk
