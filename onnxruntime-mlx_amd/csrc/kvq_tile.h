@@ -1277,7 +1277,8 @@ __device__ __forceinline__ bool slab_unit(const Params& p, int i, Unit& un, Seq&
     return un.split < un.n;
 }
 
-// New keys and values into the cache: a group of lanes per (token, kv head, key or value). Pages: the
+// New keys and values into the cache: a group of lanes per (token, kv head, key or value). 2048
+// tokens of 8 heads of 128: 9 us, the 64-bit divisions' instructions. Pages: the
 // first workgroup plans the units.
 template <int CODE, int HD, bool F32, bool PAGED>  // HD 0: any
 __global__ __launch_bounds__(256) void append_kernel(Params p) {

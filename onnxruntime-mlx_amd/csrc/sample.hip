@@ -24,6 +24,11 @@
 //                then the token by the kept weight of every 512 indices and, in the 512 that
 //                pass u, of every one.
 // A row whose border lies too low for the list has its selection over all of the row.
+//
+// Measured, each launch in turn: 1 x 151936 fp16, top-k and top-p, 2.7 + 4.4 + 8.4 + 8.5 us, all
+// latency; 32 x 128256 fp32, top-p alone, 5 + 19 + 16 + 17 (the 64-bit weights of all logits bind
+// the second: 16.4 MB at 0.9 TB/s); 256 x 151936 bf16 with settings of every kind 16 + 43 + 43 +
+// 20 (the first reads its 78 MB at 5 TB/s, the next two are vector instructions a logit).
 #include <algorithm>
 #include <cmath>
 
