@@ -495,7 +495,8 @@ int ortmi_group_query_attention_quantized(
  * cos/sin, head_sink [num_heads], q_norm_weight / k_norm_weight as ortmi_paged_attention;
  * no slot_mapping, rotary_offset or LATENT layout. Every key and value, the new ones too,
  * is read as the cache holds it; a position whose block the table does not hold
- * (an id outside the cache) is neither written nor attended. Rows of output that belong to
+ * (an id outside the cache) is neither written nor attended. Sequences may share blocks that
+ * none of them writes; two new rows at one slot leave it undefined. At most 2^31 - 4096 keys. Rows of output that belong to
  * no sequence are left as they were. The workspace holds
  * ortmi_paged_attention_quantized_workspace_size bytes.
  */

@@ -363,7 +363,7 @@ extern "C" size_t ortmi_group_query_attention_quantized_workspace_size(
     int64_t batch, int64_t seq_len, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
     int64_t total_kv) {
     if (batch <= 0 || seq_len <= 0 || kv_num_heads <= 0 || num_heads < kv_num_heads ||
-        !kvq::tile_head(head_size))
+        std::max({batch, seq_len, num_heads}) > INT32_MAX || !kvq::tile_head(head_size))
         return 0;
     size_t most = 0;  // over the types: fp32 has tiles of its own
     for (int dtype : {ORTMI_F32, ORTMI_F16}) {
@@ -395,7 +395,8 @@ extern "C" int ortmi_group_query_attention_quantized(
                               cache_type, dtype))
         return rc;
     ORTMI_REQUIRE(batch >= 0 && seq_len >= 0 && past_cap >= 0, what + ": negative size");
-    ORTMI_REQUIRE(batch * seq_len * num_heads < (1LL << 31) && past_cap + seq_len < (1LL << 31) - 4096 &&
+    ORTMI_REQUIRE(batch < (1LL << 31) && seq_len < (1LL << 31) && past_cap < (1LL << 31) &&
+                      batch * seq_len < (1LL << 31) && batch * seq_len * num_heads < (1LL << 31) && past_cap + seq_len < (1LL << 31) - 4096 &&
                       batch * kv_num_heads < (1LL << 31),
                   what + ": too many rows");
     if (batch == 0 || seq_len == 0) return ORTMI_OK;
@@ -480,7 +481,7 @@ extern "C" size_t ortmi_paged_attention_quantized_workspace_size(
     int64_t num_tokens, int64_t batch, int64_t num_heads, int64_t kv_num_heads, int64_t head_size,
     int64_t max_context) {
     if (num_tokens <= 0 || batch <= 0 || kv_num_heads <= 0 || num_heads < kv_num_heads ||
-        !kvq::tile_head(head_size))
+        std::max({num_tokens, batch, num_heads}) > INT32_MAX || !kvq::tile_head(head_size))
         return 0;
     size_t most = 0;  // over the types: fp32 has tiles of its own
     for (int dtype : {ORTMI_F32, ORTMI_F16}) {

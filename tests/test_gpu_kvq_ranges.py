@@ -135,3 +135,21 @@ def test_the_stream_of_the_call(ortmi):
     check_paged(paged, pages, pt)
     assert torch.equal(drawn, ids)
     del junk
+
+
+def test_prompts_by_the_hundred(ortmi):
+    """More sequences with prompt tiles than the GPU has CUs."""
+    new = [5 + i % 4 for i in range(300)]
+    past = [(53 * i) % 400 for i in range(300)]
+    run_paged(ortmi, past=tuple(past), new=tuple(new), H=4, KV=1, hd=64, code="int4")
+
+
+@pytest.mark.parametrize("new", [(1, 1, 1), (20, 1, 40)])
+def test_shared_prefix(ortmi, new):
+    """Sequences that read the same first blocks."""
+    args, t = make_paged(past=(70, 64, 90), new=new, hd=128, H=8, blk=16)
+    t["bt"][1:, :4] = t["bt"][0, :4]
+    args["block_table"].copy_(t["bt"])
+    out = ortmi.paged_attention_quantized(**args)
+    torch.cuda.synchronize()
+    check_paged(out, args, t)
